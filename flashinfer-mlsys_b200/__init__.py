@@ -22,9 +22,19 @@ from .binding import (  # noqa: F401
     add_rmsnorm_quantize,
     route,
 )
+from .balance import balance_loss  # noqa: F401
+from .mx import (  # noqa: F401
+    add_rmsnorm_quantize_mx,
+    dequantize_mx,
+    experts_matmul_mx,
+    matmul_mx,
+    quantize_mx,
+)
 from . import workloads  # noqa: F401
 from ._lib import MoeError, lib_path, load  # noqa: F401
 
 __all__ = [
-    "kernel", "kernel_ex", "kernel_shared", "route", "experts", "quantize_activations", "add_rmsnorm_quantize", "device_status", "last_rows", "workloads", "MoeError", "load", "lib_path",
+    "kernel", "kernel_ex", "kernel_shared", "route", "experts", "quantize_activations", "add_rmsnorm_quantize", "device_status", "last_rows",
+    "quantize_mx", "dequantize_mx", "add_rmsnorm_quantize_mx", "matmul_mx", "experts_matmul_mx", "balance_loss",
+    "workloads", "MoeError", "load", "lib_path",
 ]

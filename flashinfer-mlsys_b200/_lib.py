@@ -12,6 +12,7 @@ import threading
 from . import build as _build
 
 _c_int64 = ctypes.c_int64
+_c_int = ctypes.c_int
 _vp = ctypes.c_void_p
 
 # name -> (restype, argtypes)
@@ -47,6 +48,21 @@ SIGNATURES = {
     "moe_fp8_ds_ep_pack": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_int64, _vp, _c_int64, _vp, _vp]),
     "moe_fp8_ds_ep_unpack": (ctypes.c_int, [_vp, _c_int64, _vp, _vp, _vp, _vp, _vp]),
     "moe_fp8_ds_ep_combine": (ctypes.c_int, [_vp, _vp, _c_int64, _c_int64, _vp, _vp]),
+    "moe_fp8_ds_quantize_mx": (
+        _c_int, [_vp, _c_int, _c_int64, _c_int64, _c_int64, _c_int, _vp, _vp, _vp, _vp]),
+    "moe_fp8_ds_dequantize_mx": (
+        _c_int, [_vp, _vp, _c_int64, _c_int64, _c_int, _vp, _c_int, _vp, _c_int64, _vp]),
+    "moe_fp8_ds_add_norm_quantize_mx": (
+        _c_int, [_vp, _c_int64, _vp, _c_int64, _vp, ctypes.c_float, _c_int, _c_int64, _c_int64, _c_int, _vp, _vp, _vp, _vp]),
+    "moe_fp8_ds_matmul_mx": (
+        _c_int, [_vp] * 4 + [_c_int64] * 3 + [_c_int, _vp, _vp, _c_int, _c_int64, _vp]),
+    "moe_fp8_ds_experts_matmul_mx": (
+        _c_int, [_vp] * 5 + [_c_int64] * 4 + [_c_int, _vp, _vp, _c_int, _c_int64, _vp]),
+    "moe_fp8_ds_balance_loss_work_bytes": (ctypes.c_size_t, [_c_int64] * 3),
+    "moe_fp8_ds_balance_loss": (
+        _c_int, [_vp, _c_int, _c_int64, _vp, _vp] + [_c_int64] * 4 + [_c_int, ctypes.c_float] + [_vp] * 4),
+    "moe_fp8_ds_balance_loss_backward": (
+        _c_int, [_vp, _c_int, _c_int64, _vp, _vp] + [_c_int64] * 4 + [_c_int, ctypes.c_float] + [_vp] * 4),
     "moe_fp8_ds_ep_plan": (ctypes.c_int, [_vp, _c_int64, _c_int64, _vp, _vp, _vp, _vp]),
 }
 

@@ -17,8 +17,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libmoe_fp8_ds.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")  # moe_fp8_ds.h, the C ABI
-SOURCES = ["moe_route.cu", "moe_gemm.cu", "moe_decode.cu", "moe_quant.cu", "moe_ep.cu", "moe_api.cu", "moe_noalloc.cu"]
-HEADERS = ["moe_common.cuh", "moe_kernels.h", "moe_routing.cuh"]
+SOURCES = ["moe_route.cu", "moe_gemm.cu", "moe_decode.cu", "moe_quant.cu", "moe_ep.cu", "moe_api.cu", "moe_noalloc.cu",
+           "moe_mx_quant.cu", "moe_mx_gemm.cu", "moe_balance.cu", "moe_mx_api.cu"]
+HEADERS = ["moe_common.cuh", "moe_kernels.h", "moe_routing.cuh", "moe_mx.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

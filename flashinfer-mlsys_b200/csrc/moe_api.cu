@@ -243,6 +243,28 @@ bool fused_decode_enabled() {
 uint64_t g_test_wait_limit_ns = 0;
 int g_test_skip_arrival = -1;
 
+}  // namespace
+
+// For the entry points in moe_mx_api.cu.
+namespace moe {
+int check_device_sm100() { return check_device(); }
+
+bool encode_map_3d(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t planes,
+                   uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {cols, rows, planes};
+  const cuuint64_t strides[2] = {cols, cols * rows};
+  const cuuint32_t box[3] = {128, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace moe
+
+namespace {
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 bool valid_e_local(int64_t e) { return e == 32 || e == 64 || e == 128 || e == 256; }
@@ -563,6 +585,11 @@ int moe_fp8_ds_device_status(void* stream) {
       cudaMemset(kv.second.base, 0, kv.second.zero_bytes);
       rc = MOE_ERR_DEVICE_TIMEOUT;
     }
+  }
+  if (check_device() == MOE_OK) {
+    unsigned v = 0;
+    if (mx_take_status(&v) != cudaSuccess) return MOE_ERR_CUDA;
+    if (v) rc = MOE_ERR_DEVICE_TIMEOUT;
   }
   return rc;
 }

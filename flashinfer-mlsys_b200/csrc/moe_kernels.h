@@ -170,6 +170,74 @@ cudaError_t launch_quant_rows(const void* x, int T, void* q, float* scale, cudaS
 cudaError_t launch_add_norm_quant(const void* x, void* residual, const void* w, float eps, int T, void* q,
                                   float* scale, cudaStream_t s);
 
+// ---- microscaled formats (moe_mx.cuh: kFmt*, kDt*) ----
+cudaError_t launch_mx_quant(const void* x, int dt, int64_t x_ld, int64_t rows, int64_t cols, int fmt,
+                            const float* global_scale, void* q, void* scale, cudaStream_t s);
+cudaError_t launch_mx_dequant(const void* q, const void* scale, int64_t rows, int64_t cols, int fmt,
+                              const float* global_scale, int dt, void* x, int64_t x_ld, cudaStream_t s);
+constexpr int64_t kMxNormMaxCols = 32768;  // one thread per 32 columns, 1024 threads
+struct MxNormCall {
+  const void* x;
+  int64_t x_ld;
+  void* residual;  // or nullptr
+  int64_t res_ld;
+  const void* weight;  // or nullptr: no normalisation
+  float eps;
+  int64_t rows, cols;
+  const float* global_scale;
+  void* q;
+  void* scale;
+};
+cudaError_t launch_mx_norm(const MxNormCall& c, int fmt, int dt, cudaStream_t s);
+
+struct MxGemmCall {
+  const void* a_scale;  // [rows][K / block]
+  const void* b_scale;  // [experts][N][K / block]
+  const int32_t* off;   // [experts + 1], or nullptr: one run
+  const float* alpha;   // [experts] or nullptr
+  void* out;
+  int64_t out_ld;
+  int out_dt;
+  int experts;
+  int64_t rows, N, K;
+  int fmt;
+};
+struct MxPlan {
+  int tn;     // tokens of a tile (the token map's box rows)
+  int nt;     // kernel variant: tile room
+  int split;  // cluster size along K
+  int grid;
+};
+constexpr int kMxGemmMaxExperts = 512;
+int mx_gemm_stages(int64_t K, int fmt);
+MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs);
+// map_w: weights [experts][N][K bytes], boxes of 128 rows x 128 bytes; map_a: tokens [rows][K bytes], boxes of plan.tn rows
+cudaError_t launch_mx_gemm(const CUtensorMap& map_w, const CUtensorMap& map_a, const MxGemmCall& c, const MxPlan& pl,
+                           cudaStream_t s);
+cudaError_t mx_take_status(unsigned* v);  // reads and clears the product's status word (synchronous)
+
+// ---- balance loss (moe_balance.cu) ----
+struct BalanceCall {
+  const void* logits;
+  int dt;
+  int64_t ld;
+  const int32_t* ids;
+  const int32_t* off;  // or nullptr: one sequence
+  int64_t T;
+  int E, K, S;
+  int softmax;
+  float coeff;
+};
+int64_t balance_slots(int64_t T, int64_t S);  // scratch: 8 * E bytes each
+cudaError_t launch_balance(const BalanceCall& c, void* work, float* loss, int32_t* counts, cudaStream_t s);
+cudaError_t launch_balance_backward(const BalanceCall& c, const int32_t* counts, const float* grad_loss, void* grad,
+                                    cudaStream_t s);
+
+// ---- shared host helpers (moe_api.cu) ----
+int check_device_sm100();  // MOE_OK or MOE_ERR_NO_DEVICE
+// Byte tensor [planes][rows][cols bytes], contiguous; box 128 bytes x box_rows x 1, 128-byte swizzle.
+bool encode_map_3d(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t planes, uint32_t box_rows);
+
 size_t decode_smem_bytes();
 // map_w13: W13 [E_l*4096][7168] 128-row boxes; map_w2: W2 [E_l*7168][2048]
 // 128-row boxes; map_x1: hidden_states [T][7168] 64-row boxes (rows >= T read

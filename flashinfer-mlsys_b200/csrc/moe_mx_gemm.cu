@@ -1,0 +1,650 @@
+// moe_mx_gemm.cu — the microscaled product on the block-scaled tensor cores,
+// for one weight matrix or for one a run of rows (the experts' products):
+//   out[t, n] = alpha[e] * sum_k A[t, k] SA[t, k / blk] * W[e, n, k] SW[e, n, k / blk]
+// for the rows t of expert e, off[e] <= t < off[e + 1]. Products and block
+// scales are applied by tcgen05.mma (exact), sums are fp32, the result is
+// rounded once to the output's type. Rows outside the runs are not written.
+//
+// Weights are the M operand (128 rows a tile), tokens the N operand (16..256 a
+// tile, chosen per call): a decode call then streams whole 128-row weight
+// tiles against one narrow token tile, and a run's last tile issues only the
+// columns it has.
+//
+// Warp roles (448 threads, one CTA per SM, persistent):
+//   warp 0       TMA producer: 128 bytes of K of the weight tile and of the
+//                token tile per stage (256 4-bit or 128 8-bit values)
+//   warp 1       TMEM owner and MMA issuer: copies the stage's scales to TMEM
+//                (tcgen05.cp) and issues four K slices of 32 bytes
+//   warps 2-5    scale loaders, a stage each in turn. Scales are stored row by
+//                row; the tensor core wants, for 128 rows, word w of row r at
+//                lane r % 32, column r / 32. A lane loads the words of rows
+//                l, l + 32, l + 64, l + 96 and stores them transposed.
+//   warps 6-13   epilogue: TMEM -> registers -> global, two warps a lane quarter
+// TMEM (512 columns): two slots of scales at the top and two accumulators of
+// the tile's width below, which overlap in their middle when two do not fit;
+// the epilogue drains the shared columns first and frees them.
+// Few tiles and a long K: a cluster of up to 8 CTAs splits K, and each adds its
+// share of the tokens over the cluster's shared memory in rank order, so there
+// is no scratch, no atomics, and one answer.
+#include <atomic>
+
+#include "moe_kernels.h"
+#include "moe_mx.cuh"
+
+namespace moe {
+
+namespace {
+
+constexpr int kMxMaxExperts = kMxGemmMaxExperts;
+constexpr int kMxTileN = 128;     // weight rows of a tile
+constexpr int kMxStageK = 128;    // bytes of K of a stage
+constexpr int kMxGemmThreads = 448;
+constexpr int kMxSfWarp0 = 2, kMxSfWarps = 4;
+constexpr int kMxEpiWarp0 = 6, kMxEpiWarps = 8;
+constexpr uint64_t kMxWaitNs = 2000000000ull;  // 2 s: only reached if something is broken
+
+__device__ unsigned g_mx_status;  // kErrTimeout if a bounded wait gave up
+
+template <int kFmt, int kNT>
+struct MxCfg {
+  static constexpr int kW = kFmt == kFmtNvfp4 ? 4 : (kFmt == kFmtMxfp4 ? 2 : 1);  // scale words of a row and stage
+  static constexpr int kChunks = kNT > 128 ? 2 : 1;                               // 128-token groups of scales
+  static constexpr int kTileBytes = kMxTileN * kMxStageK;
+  static constexpr int kStageBytes = kTileBytes + kNT * kMxStageK;
+  static constexpr int kSfBytes = kW * 512 * (1 + kChunks);
+  static constexpr int kStages = kNT > 128 ? 4 : (kNT > 64 ? 6 : (kNT > 32 ? 6 : 8));
+  static constexpr int kSfCols = kW * 4 * (1 + kChunks);  // TMEM columns of one slot
+  static constexpr int kAccCols = (512 - 2 * kSfCols) & ~31;
+  static constexpr int kOwnPart = kNT <= 64;              // room for the split's partial sums beside the ring
+  static constexpr int kPartBytes = kNT * kMxTileN * 4;
+  static constexpr size_t kSmem =
+      1024 + (size_t)kStages * (kStageBytes + kSfBytes) + (kOwnPart ? kPartBytes : 0);
+  static_assert(kOwnPart || kPartBytes <= kStages * kStageBytes, "partial sums reuse the ring");
+};
+
+struct MxGemmArgs {
+  const uint8_t* sa;   // [R][nsc]
+  const uint8_t* sw;   // [E][N][nsc]
+  const int32_t* off;  // [E + 1], or nullptr: one run of R rows
+  const float* alpha;  // [E] or nullptr
+  void* out;
+  int64_t out_ld;
+  int out_dt;
+  int E, R, N;
+  int nsc;             // scales of a row
+  int nk;              // stages of K
+  int tn;              // tokens of a tile (multiple of 16, <= kNT)
+  int split;           // CTAs of a cluster, each with its share of K
+};
+
+struct __align__(16) MxCtl {
+  uint64_t full[8], empty[8], tfull[2], acc_free, part_ready, part_free, mma_done;
+  uint32_t tmem_base;
+  int abort_flag;
+  int start[kMxMaxExperts + 1];   // first row of each run
+  int count[kMxMaxExperts];       // rows of each run
+  int prefix[kMxMaxExperts + 1];  // first token tile of each run
+};
+
+struct MxUnit {
+  int e, n0, row0, cnt;
+};
+
+__device__ __forceinline__ MxUnit mx_unit(const MxCtl* c, const MxGemmArgs& p, int u, int ntn) {
+  MxUnit x;
+  const int g = u / ntn;
+  x.n0 = (u - g * ntn) * kMxTileN;
+  int lo = 0, hi = p.E - 1;
+  while (lo < hi) {  // last run whose first tile is <= g (empty runs share prefixes)
+    const int mid = (lo + hi + 1) >> 1;
+    if (c->prefix[mid] <= g) lo = mid; else hi = mid - 1;
+  }
+  x.e = lo;
+  const int j = (g - c->prefix[lo]) * p.tn;
+  x.row0 = c->start[lo] + j;
+  x.cnt = min(p.tn, c->count[lo] - j);
+  return x;
+}
+
+__device__ __forceinline__ void mx_abort(MxCtl* c) {
+  atomicOr(&g_mx_status, kErrTimeout);
+  *reinterpret_cast<volatile int*>(&c->abort_flag) = 1;
+}
+__device__ __forceinline__ bool mx_aborted(MxCtl* c) { return *reinterpret_cast<volatile int*>(&c->abort_flag) != 0; }
+
+// Both operands' maps have three dimensions (bytes of a row, rows, planes).
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// 32 rows x 16 bytes of shared memory (rows 16 bytes apart) to 4 TMEM columns
+// of lanes 0-31, repeated in the other three lane quarters.
+__device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128u >> 4) << 16;  // leading offset (one 16-byte column only: unused)
+  d |= static_cast<uint64_t>(128u >> 4) << 32;  // 128 B between 8-row groups
+  d |= static_cast<uint64_t>(1u) << 46;         // descriptor version, no swizzle
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+// Instruction descriptor of the block-scaled kinds, A and B K-major, M = 128:
+// scale id of B in [4,6), type of A in [7,10) and of B in [10,13) (e2m1 = 1 in
+// the 4-bit kinds, e4m3 = 0 in mxf8f6f4), N >> 3 in [17,23), scale type bit 23
+// (0 e4m3, 1 e8m0), M >> 7 in [27,29), scale id of A in [29,31). The scale id
+// is the byte of the 32-bit scale word that holds the K slice's first scale.
+template <int kFmt>
+__device__ __forceinline__ uint32_t mx_idesc(int n, uint32_t id) {
+  const uint32_t type = kFmt == kFmtMxfp8 ? 0u : 1u;
+  const uint32_t scale = kFmt == kFmtNvfp4 ? 0u : 1u;
+  return (id << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (scale << 23) | (1u << 27) |
+         (id << 29);
+}
+
+template <int kFmt>
+__device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                       uint32_t acc) {
+  if constexpr (kFmt == kFmtNvfp4) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+  } else if constexpr (kFmt == kFmtMxfp4) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+  }
+}
+
+// ---- cluster helpers --------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive_remote(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    if (global_timer_ns() - t0 > limit_ns) return false;
+  }
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void epi_bar_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+static_assert(kMxEpiWarps * 32 == 256, "epi_bar_sync counts the epilogue's threads");
+
+__device__ __forceinline__ void mx_out_store(const MxGemmArgs& p, int64_t row, int n, float v) {
+  const int64_t i = row * p.out_ld + n;
+  if (p.out_dt == kDtBf16)
+    static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
+  else if (p.out_dt == kDtFp16)
+    static_cast<__half*>(p.out)[i] = __float2half_rn(v);
+  else
+    static_cast<float*>(p.out)[i] = v;
+}
+
+// ---- scales of up to 128 rows into the tensor core's order --------------------
+// `base`: the first row's scales at the stage's first scale; `left`: scales of
+// a row from there on. mode 2: rows are whole words, vector loads; 1: words;
+// 0: bytes (any row length).
+template <int kW>
+__device__ __forceinline__ void mx_sf_load(const uint8_t* base, int64_t nsc, int rows, int left, int mode, int lane,
+                                           uint32_t (&w)[4][kW]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = lane + 32 * j;
+#pragma unroll
+    for (int i = 0; i < kW; ++i) w[j][i] = 0;
+    if (r >= rows) continue;
+    const uint8_t* s = base + r * nsc;
+    if (mode == 2) {
+      if constexpr (kW == 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
+        w[j][0] = v.x, w[j][1] = v.y, w[j][2] = v.z, w[j][3] = v.w;
+      } else if constexpr (kW == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+        w[j][0] = v.x, w[j][1] = v.y;
+      } else {
+        w[j][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+      }
+    } else if (mode == 1) {
+#pragma unroll
+      for (int i = 0; i < kW; ++i)
+        if (4 * i < left) w[j][i] = __ldg(reinterpret_cast<const uint32_t*>(s) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4 * kW; ++i)
+        if (i < left) w[j][i / 4] |= static_cast<uint32_t>(__ldg(s + i)) << (8 * (i % 4));
+    }
+  }
+}
+template <int kW>
+__device__ __forceinline__ void mx_sf_store(uint8_t* dst, int word_stride, int lane, const uint32_t (&w)[4][kW]) {
+#pragma unroll
+  for (int i = 0; i < kW; ++i)
+    *reinterpret_cast<uint4*>(dst + i * word_stride + lane * 16) = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
+}
+
+template <int kFmt, int kNT>
+__global__ void __launch_bounds__(kMxGemmThreads, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                   const MxGemmArgs p) {
+  using Cfg = MxCfg<kFmt, kNT>;
+  constexpr int kS = Cfg::kStages, kW = Cfg::kW;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ MxCtl ctl_;
+  MxCtl* ctl = &ctl_;
+  uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sfs = tiles + kS * Cfg::kStageBytes;
+  float* part = reinterpret_cast<float*>(Cfg::kOwnPart ? sfs + kS * Cfg::kSfBytes : tiles);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ntn = (p.N + kMxTileN - 1) / kMxTileN;
+  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
+  const int u_first = blockIdx.x / p.split, u_step = gridDim.x / p.split;
+  const int k0 = static_cast<int>((static_cast<int64_t>(p.nk) * rank) / p.split);
+  const int k1 = static_cast<int>((static_cast<int64_t>(p.nk) * (rank + 1)) / p.split);
+
+  if (tid == 0) {
+    for (int s = 0; s < kS; ++s) {
+      mbar_init(&ctl->full[s], 2);   // the TMA thread and the scale warp
+      mbar_init(&ctl->empty[s], 1);
+    }
+    mbar_init(&ctl->tfull[0], 1);
+    mbar_init(&ctl->tfull[1], 1);
+    mbar_init(&ctl->acc_free, kMxEpiWarps);
+    mbar_init(&ctl->part_ready, p.split);
+    mbar_init(&ctl->part_free, p.split);
+    mbar_init(&ctl->mma_done, 1);
+    ctl->abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_a);
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  // runs and their token tiles: one warp, 32 experts at a time
+  if (warp == 2) {
+    int base = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + lane;
+      int lo = 0, hi = 0;
+      if (e < p.E) {
+        if (p.off) {  // kept inside [0, R] whatever the offsets hold
+          lo = min(max(__ldg(p.off + e), 0), p.R);
+          hi = min(max(__ldg(p.off + e + 1), lo), p.R);
+        } else {
+          hi = p.R;
+        }
+        ctl->start[e] = lo;
+        ctl->count[e] = hi - lo;
+      }
+      const int t = (hi - lo + p.tn - 1) / p.tn;
+      int inc = t;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (e < p.E) ctl->prefix[e] = base + inc - t;
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) ctl->prefix[p.E] = base;
+  }
+  tc_fence_before();
+  if (p.split > 1)
+    cluster_sync_all();  // the barriers of every CTA of the cluster are set up
+  else
+    __syncthreads();
+  tc_fence_after();
+  const int units = ctl->prefix[p.E] * ntn;
+  const uint32_t tmem = ctl->tmem_base;
+  const int acc1 = (Cfg::kAccCols - p.tn) & ~31;  // first column of the second accumulator
+  const uint32_t acc_at[2] = {tmem, tmem + acc1};
+  const uint32_t sf_at = tmem + Cfg::kAccCols;
+
+  if (warp == 0) {
+    // ======================= TMA producer =======================
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
+        const MxUnit x = mx_unit(ctl, p, u, ntn);
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % kS;
+          if (!mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs)) { mx_abort(ctl); break; }
+          uint8_t* st = tiles + s * Cfg::kStageBytes;
+          mbar_arrive_expect_tx(&ctl->full[s], Cfg::kTileBytes + p.tn * kMxStageK);
+          tma_load_3d(st, &map_w, k * kMxStageK, x.n0, x.e, &ctl->full[s]);
+          tma_load_3d(st + Cfg::kTileBytes, &map_a, k * kMxStageK, x.row0, 0, &ctl->full[s]);
+        }
+      }
+      if (mx_aborted(ctl)) {
+        // wait (bounded) for the copies this thread may still have in flight
+        for (uint32_t j = it > (uint32_t)kS ? it - kS : 0; j < it; ++j)
+          mbar_wait_bounded(&ctl->full[j % kS], (j / kS) & 1u, kMxWaitNs);
+      }
+    }
+  } else if (warp == 1) {
+    // ======================= MMA issuer =======================
+    if (lane == 0) {
+      uint32_t it = 0, tile = 0;
+      for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step, ++tile) {
+        const MxUnit x = mx_unit(ctl, p, u, ntn);
+        const int nmma = (x.cnt + 15) & ~15;
+        const uint32_t d = acc_at[tile & 1u];
+        // the tile before last has left this accumulator and the last one the columns they share
+        if (tile > 0 && !mbar_wait_bounded(&ctl->acc_free, (tile - 1) & 1u, kMxWaitNs)) { mx_abort(ctl); break; }
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % kS;
+          // the scale slot's last readers have finished (two stages back)
+          if (it >= 2 && !mbar_wait_bounded(&ctl->empty[(it - 2) % kS], ((it - 2) / kS) & 1u, kMxWaitNs)) { mx_abort(ctl); break; }
+          if (!mbar_wait_bounded(&ctl->full[s], (it / kS) & 1u, kMxWaitNs)) { mx_abort(ctl); break; }
+          tc_fence_after();
+          const uint32_t sf = smem_u32(sfs + s * Cfg::kSfBytes);
+          const uint32_t t_w = sf_at + (it & 1u) * Cfg::kSfCols, t_a = t_w + 4 * kW;
+#pragma unroll
+          for (int i = 0; i < kW; ++i) {
+            tmem_cp_sf(t_w + 4 * i, sf + i * 512);
+#pragma unroll
+            for (int c = 0; c < Cfg::kChunks; ++c)
+              if (c * 128 < nmma)
+                tmem_cp_sf(t_a + (i * Cfg::kChunks + c) * 4, sf + kW * 512 + (i * Cfg::kChunks + c) * 512);
+          }
+          const uint32_t st = smem_u32(tiles + s * Cfg::kStageBytes);
+          const uint64_t dw = smem_desc_sw128(st), da = smem_desc_sw128(st + Cfg::kTileBytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // slice j's scales: all four bytes of word j (nvfp4), half j % 2 of word j / 2 (mxfp4), byte j (mxfp8)
+            const int word = kFmt == kFmtNvfp4 ? j : (kFmt == kFmtMxfp4 ? j / 2 : 0);
+            const uint32_t id = kFmt == kFmtNvfp4 ? 0u : (kFmt == kFmtMxfp4 ? 2u * (j % 2) : j);
+            mx_mma<kFmt>(d, dw + 2 * j, da + 2 * j, mx_idesc<kFmt>(nmma, id), t_w + 4 * word,
+                         t_a + word * Cfg::kChunks * 4, (k > k0 || j > 0) ? 1u : 0u);
+          }
+          mma_commit(&ctl->empty[s]);
+        }
+        if (mx_aborted(ctl)) break;
+        mma_commit(&ctl->tfull[tile & 1u]);
+      }
+      if (mx_aborted(ctl) && it > 0) {
+        mma_commit(&ctl->mma_done);
+        mbar_wait_bounded(&ctl->mma_done, 0, kMxWaitNs);
+      }
+    }
+  } else if (warp < kMxSfWarp0 + kMxSfWarps) {
+    // ======================= scale loaders =======================
+    const int me = warp - kMxSfWarp0;
+    const auto mode_of = [&](const uint8_t* b) {
+      const uint64_t m = reinterpret_cast<uint64_t>(b) | static_cast<uint64_t>(p.nsc);
+      return (m & (4 * kW - 1)) == 0 ? 2 : ((m & 3) == 0 ? 1 : 0);
+    };
+    const int mode_w = mode_of(p.sw), mode_a = mode_of(p.sa);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step) {
+      const MxUnit x = mx_unit(ctl, p, u, ntn);
+      const uint8_t* bw = p.sw + (static_cast<int64_t>(x.e) * p.N + x.n0) * p.nsc;
+      const uint8_t* ba = p.sa + static_cast<int64_t>(x.row0) * p.nsc;
+      for (int k = k0; k < k1; ++k, ++it) {
+        if (static_cast<int>(it % kMxSfWarps) != me) continue;
+        const int s = it % kS;
+        const int at = k * 4 * kW, left = p.nsc - at;
+        uint32_t w[4][kW], a[Cfg::kChunks][4][kW];
+        // global loads first: they need no free stage
+        mx_sf_load<kW>(bw + at, p.nsc, p.N - x.n0, left, mode_w, lane, w);
+#pragma unroll
+        for (int c = 0; c < Cfg::kChunks; ++c)
+          mx_sf_load<kW>(ba + at + static_cast<int64_t>(c) * 128 * p.nsc, p.nsc, x.cnt - c * 128, left, mode_a, lane, a[c]);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs));
+        if (!ok) { mx_abort(ctl); break; }
+        uint8_t* sf = sfs + s * Cfg::kSfBytes;
+        mx_sf_store<kW>(sf, 512, lane, w);
+#pragma unroll
+        for (int c = 0; c < Cfg::kChunks; ++c) mx_sf_store<kW>(sf + kW * 512 + c * 512, Cfg::kChunks * 512, lane, a[c]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->full[s]);
+      }
+    }
+  } else {
+    // ======================= epilogue (8 warps) =======================
+    const int q = warp & 3, half = (warp - kMxEpiWarp0) >> 2;
+    const uint32_t t_lane = static_cast<uint32_t>(q * 32) << 16;
+    const int etid = tid - kMxEpiWarp0 * 32;
+    const int nl = q * 32 + lane;  // weight row of this thread inside the tile
+    const int nch = p.tn / 16;
+    const int shared_cols = p.tn - acc1;
+    const int ovc = shared_cols > 0 ? (shared_cols + 15) / 16 : 0;
+    uint32_t tile = 0;
+    for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step, ++tile) {
+      const MxUnit x = mx_unit(ctl, p, u, ntn);
+      const uint32_t buf = tile & 1u;
+      const float alpha = p.alpha ? __ldg(p.alpha + x.e) : 1.0f;
+      if (p.split > 1 && tile > 0) {  // the cluster has read this CTA's last partial sums
+        if (!__all_sync(0xffffffffu, cluster_wait_bounded(&ctl->part_free, (tile - 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctl->tfull[buf], (tile >> 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+      __syncwarp();
+      tc_fence_after();
+      bool freed = false;
+      // buffer 0 shares its last columns with buffer 1's first
+      for (int i = half; i < nch; i += 2) {
+        if (!freed && i >= ovc) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->acc_free);
+          freed = true;
+        }
+        const int c = (buf == 0 ? nch - 1 - i : i) * 16;
+        if (c >= x.cnt) continue;
+        float v[16];
+        tmem_ld_32x32b_x16(acc_at[buf] + t_lane + c, v);
+        if (p.split > 1) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(c + j) * kMxTileN + nl] = v[j];
+        } else if (x.n0 + nl < p.N) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c + j < x.cnt) mx_out_store(p, static_cast<int64_t>(x.row0) + c + j, x.n0 + nl, v[j] * alpha);
+        }
+      }
+      if (!freed) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->acc_free);
+      }
+      if (p.split > 1) {
+        epi_bar_sync();
+        if (etid < p.split) cluster_arrive_remote(cluster_map(smem_u32(&ctl->part_ready), etid));
+        if (!__all_sync(0xffffffffu, cluster_wait_bounded(&ctl->part_ready, tile & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+        // tokens rank, rank + split, ...: a warp a token, four weight rows a lane
+        const int n = x.n0 + lane * 4;
+        for (int t = rank + (warp - kMxEpiWarp0) * p.split; t < x.cnt; t += kMxEpiWarps * p.split) {
+          const uint32_t at = smem_u32(part + t * kMxTileN + lane * 4);
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int r = 0; r < p.split; ++r) {
+            const float4 v = ld_cluster_f4(cluster_map(at, r));
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+          }
+          const int64_t row = static_cast<int64_t>(x.row0) + t;
+          if (n < p.N) mx_out_store(p, row, n, sum.x * alpha);
+          if (n + 1 < p.N) mx_out_store(p, row, n + 1, sum.y * alpha);
+          if (n + 2 < p.N) mx_out_store(p, row, n + 2, sum.z * alpha);
+          if (n + 3 < p.N) mx_out_store(p, row, n + 3, sum.w * alpha);
+        }
+        epi_bar_sync();
+        if (etid < p.split) cluster_arrive_remote(cluster_map(smem_u32(&ctl->part_free), etid));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  if (p.split > 1)
+    cluster_sync_all();  // no CTA leaves while another may read its sums
+  else
+    __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int kFmt, int kNT>
+cudaError_t mx_gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const MxGemmArgs& p, int grid, cudaStream_t s) {
+  using Cfg = MxCfg<kFmt, kNT>;
+  static_assert(Cfg::kSmem + sizeof(MxCtl) <= 232448, "shared memory of a CTA");
+  // the shared-memory opt-in is an attribute of the function on a device: one bit per device that has it
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(configured.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(mx_gemm_kernel<kFmt, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Cfg::kSmem));
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kMxGemmThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<kFmt, kNT>, mw, ma, p);
+}
+
+template <int kFmt>
+cudaError_t mx_gemm_launch_nt(int nt, const CUtensorMap& mw, const CUtensorMap& ma, const MxGemmArgs& p, int grid,
+                              cudaStream_t s) {
+  switch (nt) {
+    case 32: return mx_gemm_launch<kFmt, 32>(mw, ma, p, grid, s);
+    case 64: return mx_gemm_launch<kFmt, 64>(mw, ma, p, grid, s);
+    case 128: return mx_gemm_launch<kFmt, 128>(mw, ma, p, grid, s);
+    default: return mx_gemm_launch<kFmt, 256>(mw, ma, p, grid, s);
+  }
+}
+
+}  // namespace
+
+// Tokens of a tile, K split and grid of a call.
+// One run of rows: the tile width that gives the least (waves of CTAs) x
+// (rows loaded per stage). Several runs, whose lengths only the device knows:
+// by their mean length.
+MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs) {
+  const int sms = device_sm_count();
+  const int64_t ntn = (N + kMxTileN - 1) / kMxTileN;
+  MxPlan pl{};
+  if (runs) {
+    const int64_t mean = (rows + experts - 1) / experts;
+    pl.tn = mean <= 8 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 160 ? 128 : 256;
+  } else if (rows <= 64) {
+    pl.tn = static_cast<int>((rows + 15) / 16 * 16);
+  } else {
+    int64_t best = INT64_MAX;
+    for (int tn = 64; tn <= 256; tn += 16) {
+      const int64_t waves = (((rows + tn - 1) / tn) * ntn + sms - 1) / sms;
+      const int64_t cost = waves * (kMxTileN + tn);
+      if (cost <= best) {
+        best = cost;
+        pl.tn = tn;
+      }
+    }
+  }
+  pl.nt = pl.tn <= 32 ? 32 : pl.tn <= 64 ? 64 : pl.tn <= 128 ? 128 : 256;
+  const int64_t busy = runs ? (experts < rows ? experts : rows) : 1;             // runs that can have rows
+  const int64_t most = (rows / pl.tn + busy) * ntn;                              // no call has more tiles
+  const int64_t tiles = runs ? most : (rows + pl.tn - 1) / pl.tn * ntn;
+  pl.split = 1;
+  while (pl.split < 8 && tiles * pl.split * 2 <= sms && nk >= 4 * pl.split) pl.split *= 2;
+  if (runs && pl.nt > 64) pl.split = 1;  // a cluster with several tiles needs its own room for partial sums
+  const int64_t groups = tiles < sms / pl.split ? tiles : sms / pl.split;
+  pl.grid = static_cast<int>(groups) * pl.split;
+  return pl;
+}
+
+cudaError_t launch_mx_gemm(const CUtensorMap& map_w, const CUtensorMap& map_a, const MxGemmCall& c, const MxPlan& pl,
+                           cudaStream_t s) {
+  MxGemmArgs p{};
+  p.sa = static_cast<const uint8_t*>(c.a_scale);
+  p.sw = static_cast<const uint8_t*>(c.b_scale);
+  p.off = c.off;
+  p.alpha = c.alpha;
+  p.out = c.out;
+  p.out_ld = c.out_ld;
+  p.out_dt = c.out_dt;
+  p.E = c.experts;
+  p.R = static_cast<int>(c.rows);
+  p.N = static_cast<int>(c.N);
+  p.nsc = static_cast<int>(c.K / mx_block(c.fmt));
+  p.nk = mx_gemm_stages(c.K, c.fmt);
+  p.tn = pl.tn;
+  p.split = pl.split;
+  switch (c.fmt) {
+    case kFmtNvfp4: return mx_gemm_launch_nt<kFmtNvfp4>(pl.nt, map_w, map_a, p, pl.grid, s);
+    case kFmtMxfp4: return mx_gemm_launch_nt<kFmtMxfp4>(pl.nt, map_w, map_a, p, pl.grid, s);
+    default: return mx_gemm_launch_nt<kFmtMxfp8>(pl.nt, map_w, map_a, p, pl.grid, s);
+  }
+}
+
+int mx_gemm_stages(int64_t K, int fmt) {
+  const int64_t bytes = fmt == kFmtMxfp8 ? K : K / 2;
+  return static_cast<int>((bytes + kMxStageK - 1) / kMxStageK);
+}
+
+cudaError_t mx_take_status(unsigned* v) {
+  cudaError_t e = cudaMemcpyFromSymbol(v, g_mx_status, 4);
+  if (e == cudaSuccess && *v) {
+    const unsigned zero = 0;
+    e = cudaMemcpyToSymbol(g_mx_status, &zero, 4);
+  }
+  return e;
+}
+
+}  // namespace moe

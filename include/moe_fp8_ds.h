@@ -260,6 +260,107 @@ int moe_fp8_ds_ep_plan(const int32_t* topk_ids, int64_t seq_len, int64_t world, 
 int moe_fp8_ds_ep_combine(const void* partials, const int32_t* row_of, int64_t seq_len, int64_t world, void* output,
                           void* stream);
 
+/*
+ * ---- Microscaled operators ----------------------------------------------
+ * Values in blocks along a row, one scale a block, as the block-scaled tensor
+ * cores read them (no counterpart in the reference, whose layer uses e4m3
+ * with fp32 scales per 128 values):
+ *   MOE_MX_NVFP4  e2m1 values, blocks of 16, e4m3 scales, one fp32 scale of
+ *                 the tensor (global_scale, a device pointer; NULL = 1)
+ *   MOE_MX_MXFP4  e2m1 values, blocks of 32, e8m0 scales (2^(byte - 127))
+ *   MOE_MX_MXFP8  e4m3 values, blocks of 32, e8m0 scales
+ * e2m1 values are packed two a byte, the even column in the low half; packed
+ * rows and rows of scales are contiguous. cols (and k below) are multiples of
+ * 32. Rows of bf16/fp16/fp32 tensors lie `*_ld` elements apart and are 16-byte
+ * aligned.
+ *
+ * Quantisation rule, float32 throughout, every rounding to nearest even:
+ *   nvfp4  s = e4m3(min(448, amax / (6 g))), q = e2m1(x / (s g)); 0 where s g = 0
+ *   mx     s = 2^clamp(floor(log2 amax) - emax, -127, 127), emax 2 (e2m1) or 8
+ *          (e4m3), q = round(x / s), saturating
+ *   A block with an infinity or a NaN gets a NaN scale and zeros.
+ * global_scale must be positive and finite.
+ */
+#define MOE_MX_NVFP4 0
+#define MOE_MX_MXFP4 1
+#define MOE_MX_MXFP8 2
+#define MOE_DT_BF16 0
+#define MOE_DT_FP16 1
+#define MOE_DT_FP32 2
+
+/* x [rows][cols] -> q_out, scale_out. */
+int moe_fp8_ds_quantize_mx(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_ld, int fmt,
+                           const float* global_scale, void* q_out, void* scale_out, void* stream);
+
+/* x_out = (value * scale) * global_scale, rounded once to dtype. */
+int moe_fp8_ds_dequantize_mx(const void* q, const void* scale, int64_t rows, int64_t cols, int fmt,
+                             const float* global_scale, int dtype, void* x_out, int64_t x_ld, void* stream);
+
+/*
+ * The decoder's residual add, RMSNorm and quantisation in one pass, for any
+ * width up to 32768 (moe_fp8_ds_add_norm_quant is the 7168-wide form with
+ * 1x128 fp32 scales):
+ *   h = dtype(residual + x)                    written back to residual
+ *   y = h / sqrt(mean(h^2) + eps) * weight     in float32
+ *   q_out, scale_out = the quantisation of y
+ * residual NULL: h = x. norm_weight (dtype, [cols]) NULL: y = h.
+ */
+int moe_fp8_ds_add_norm_quantize_mx(const void* x, int64_t x_ld, void* residual, int64_t residual_ld,
+                                    const void* norm_weight, float eps, int dtype, int64_t rows, int64_t cols, int fmt,
+                                    const float* global_scale, void* q_out, void* scale_out, void* stream);
+
+/*
+ * out[i][j] = alpha * sum over k of a[i][k] a_scale * b[j][k] b_scale, fp32
+ * sums, rounded once to out_dtype; a [m][k], b [n][k] packed in `fmt`. alpha:
+ * a device pointer (the product of the tensors' global scales) or NULL = 1.
+ * Scale bytes are read as unsigned: e4m3 scales must not be negative.
+ * m <= 2^24, n <= 2^18, k <= 2^20.
+ */
+int moe_fp8_ds_matmul_mx(const void* a, const void* a_scale, const void* b, const void* b_scale, int64_t m, int64_t n,
+                         int64_t k, int fmt, const float* alpha, void* out, int out_dtype, int64_t out_ld,
+                         void* stream);
+
+/*
+ * The same with one weight matrix a run of rows: rows expert_offsets[e] ..
+ * expert_offsets[e + 1] - 1 of a (int32 [num_experts + 1] on the device, not
+ * decreasing; values are kept inside [0, m]) use b[e] ([num_experts][n][k])
+ * and alpha[e]. Rows outside the runs are left as they were. num_experts <= 512.
+ */
+int moe_fp8_ds_experts_matmul_mx(const void* a, const void* a_scale, const void* b, const void* b_scale,
+                                 const int32_t* expert_offsets, int64_t num_experts, int64_t m, int64_t n, int64_t k,
+                                 int fmt, const float* alpha, void* out, int out_dtype, int64_t out_ld, void* stream);
+
+/*
+ * ---- Balance loss of the router -------------------------------------------
+ * DeepSeek-V3's sequence-wise balance loss with the per-expert counts (no
+ * counterpart in the reference, which has no training step). Sequence s is
+ * tokens seq_offsets[s] .. seq_offsets[s + 1] - 1 (int32 [seqs + 1] on the
+ * device, not decreasing; NULL with seqs = 1: all tokens), T_s of them:
+ *   f_i  = experts / (topk T_s) * number of slots of the sequence with id i
+ *   p_ti = score(logit_ti) / sum_j score(logit_tj), score = sigmoid or exp
+ *   loss_out[s] = coeff * sum_i f_i * mean_t p_ti      (0 for an empty sequence)
+ *   counts_out int32 [seqs][experts]: slots of the sequence with that id
+ * Ids outside [0, experts) are not counted; an id that occurs twice counts
+ * twice. A token whose scores sum to zero in float32 has p = 0.
+ * logits [tokens][experts] of dtype, rows logits_ld apart; topk_ids int32
+ * [tokens][topk]; work: device scratch of moe_fp8_ds_balance_loss_work_bytes
+ * bytes, any content. The backward call writes
+ * d(sum_s grad_loss[s] loss[s]) / d logits (contiguous, dtype; counts carry no
+ * gradient; tokens of no sequence get zeros) from the forward call's counts.
+ * Results do not depend on scheduling.
+ */
+#define MOE_SCORE_SIGMOID 0
+#define MOE_SCORE_SOFTMAX 1
+#define MOE_BALANCE_MAX_EXPERTS 1024
+size_t moe_fp8_ds_balance_loss_work_bytes(int64_t tokens, int64_t experts, int64_t seqs);
+int moe_fp8_ds_balance_loss(const void* routing_logits, int dtype, int64_t logits_ld, const int32_t* topk_ids,
+                            const int32_t* seq_offsets, int64_t tokens, int64_t experts, int64_t topk, int64_t seqs,
+                            int score, float coeff, void* work, float* loss_out, int32_t* counts_out, void* stream);
+int moe_fp8_ds_balance_loss_backward(const void* routing_logits, int dtype, int64_t logits_ld, const int32_t* topk_ids,
+                                     const int32_t* seq_offsets, int64_t tokens, int64_t experts, int64_t topk,
+                                     int64_t seqs, int score, float coeff, const int32_t* counts,
+                                     const float* grad_loss, void* grad_logits_out, void* stream);
+
 /* Human-readable text for a status code (static storage, never NULL). */
 const char* moe_fp8_ds_status_string(int status);
 

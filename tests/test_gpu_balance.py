@@ -1,0 +1,169 @@
+"""GPU: the router's balance loss, its counts and its gradient, against
+float64 on the CPU and against differences."""
+import pytest
+import torch
+
+import mx_reference as R
+from conftest import pkg
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def _inputs(T, E, K, S, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, E, generator=g) + 0.5 * torch.randn(E, generator=g)
+    ids = (x.topk(K, 1).indices if T else torch.zeros(0, K)).int()
+    cut = torch.randint(0, T + 1, (S - 1,), generator=g).sort().values
+    off = torch.cat((torch.zeros(1), cut, torch.full((1,), float(T)))).int()
+    return x.to(dtype), ids, off, torch.rand(S, generator=g) + 0.5
+
+
+def _check(x, ids, off, grad, score, coeff=0.3):
+    xd = x.to(DEV).requires_grad_(True)
+    offd = None if off is None else off.to(DEV)
+    loss, counts = pkg().balance_loss(xd, ids.to(DEV), offd, coeff, score)
+    dx, = torch.autograd.grad(loss, xd, grad.to(DEV))
+    want, n, back = R.balance(x.float(), ids, off, coeff, score)
+    assert counts.dtype == torch.int32 and torch.equal(counts.cpu().long(), n)
+    assert loss.dtype == torch.float32 and loss.shape == want.shape
+    # a score: exp (2 steps), add, divide; the row's sum (log2 E + E / 32 adds), the reciprocal and product; a
+    # column's sum of a run's tokens; each at most 2^-24 of the value (every term is positive): under 128 of them
+    # and one for each 64 tokens of a run
+    T, E = x.shape
+    rel = (128 + E / 32 + T / 64) * 2.0 ** -24
+    torch.testing.assert_close(loss.cpu().double(), want, rtol=rel, atol=0)
+    # d = g c / T_s p_j (f_j - sum f p) (..): the difference cancels, so the error is relative to its two terms
+    assert dx.dtype == x.dtype and dx.shape == x.shape
+    off_l = [0, T] if off is None else off.tolist()
+    ref = back(grad)
+    tol = torch.zeros(T, E, dtype=torch.float64)
+    for s, (lo, hi) in enumerate(zip(off_l[:-1], off_l[1:])):
+        if hi > lo:
+            r = x[lo:hi].double()
+            p = torch.softmax(r, 1) if score == "softmax" else r.sigmoid() / r.sigmoid().sum(1, keepdim=True)
+            f = n[s].double() * E / (ids.shape[1] * (hi - lo))
+            tol[lo:hi] = rel * grad[s].double() * coeff / (hi - lo) * p * (f + (p * f).sum(1, keepdim=True))
+    tol += torch.finfo(x.dtype).eps / 2 * 1.01 * ref.abs() + torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps
+    assert ((dx.cpu().double() - ref).abs() <= tol).all()
+    return loss, dx
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T,E,K,S,dtype", [
+    (1, 256, 8, 1, "fp32"), (7, 8, 2, 3, "fp32"), (1000, 256, 8, 5, "fp32"), (1000, 256, 8, 40, "bf16"),
+    (333, 60, 4, 7, "fp16"), (129, 1, 1, 2, "fp32"), (50, 1024, 8, 3, "fp32"), (77, 513, 6, 4, "bf16"),
+    (9000, 64, 6, 2, "fp32"), (5, 160, 6, 64, "fp32")])
+def test_balance_loss(gpu_available, score, T, E, K, S, dtype):
+    _check(*_inputs(T, E, K, S, R.DTYPES[dtype], T + E + S), score)
+
+
+def test_one_sequence_without_offsets_and_strided_logits(gpu_available):
+    x, ids, _, grad = _inputs(100, 96, 4, 1, torch.float32, 3)
+    _check(x, ids, None, grad, "sigmoid")
+    wide = torch.zeros(100, 131)
+    wide[:, 17:113] = x
+    view = wide.to(DEV)[:, 17:113].requires_grad_(True)
+    loss, _ = pkg().balance_loss(view, ids.to(DEV), None, 0.3)
+    want, _, back = R.balance(x, ids, None, 0.3, "sigmoid")
+    torch.testing.assert_close(loss.detach().cpu().double(), want, rtol=2.0 ** -16, atol=0)
+    dx, = torch.autograd.grad(loss.sum(), view)
+    assert dx.shape == x.shape
+    torch.testing.assert_close(dx.cpu().double(), back(torch.ones(1)), rtol=1e-3, atol=1e-9)
+
+
+def test_ids_outside_repeated_and_tokens_of_no_sequence(gpu_available):
+    x, ids, _, _ = _inputs(64, 32, 4, 1, torch.float32, 4)
+    ids[3] = torch.tensor([-1, 32, 1 << 30, -(1 << 31)])
+    ids[4] = 7
+    off = torch.tensor([5, 20, 20, 50], dtype=torch.int32)
+    _, dx = _check(x, ids, off, torch.tensor([1.0, 2.0, 0.5]), "softmax")
+    assert (dx[:5] == 0).all() and (dx[50:] == 0).all() and (dx[5:50] != 0).any()
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_masked_logits(gpu_available, score):
+    """-inf in places, a row of them, the type's lowest value, a NaN row."""
+    x, ids, off, grad = _inputs(40, 64, 4, 2, torch.float32, 5)
+    x[1, :60] = -torch.inf
+    x[2] = -torch.inf
+    x[3, 5] = torch.finfo(torch.float32).min
+    xd = x.to(DEV).requires_grad_(True)
+    loss, counts = pkg().balance_loss(xd, ids.to(DEV), off.to(DEV), 1.0, score)
+    dx, = torch.autograd.grad(loss, xd, grad.to(DEV))
+    assert loss.isfinite().all() and dx.isfinite().all() and (dx[2] == 0).all() and (dx[1, :60] == 0).all()
+    keep = torch.ones(40, dtype=torch.bool)
+    keep[2] = False
+    # without the empty row's terms: its p is 0 and its ids still count
+    y = x.double()[keep]
+    p = torch.zeros(40, 64, dtype=torch.float64)
+    p[keep] = torch.softmax(y, 1) if score == "softmax" else y.sigmoid() / y.sigmoid().sum(1, keepdim=True)
+    for s in range(2):
+        lo, hi = int(off[s]), int(off[s + 1])
+        if hi > lo:
+            f = counts[s].cpu().double() * 64 / (4 * (hi - lo))
+            want = (f * p[lo:hi].sum(0) / (hi - lo)).sum()
+            torch.testing.assert_close(loss[s].detach().cpu().double(), want, rtol=2.0 ** -16, atol=0)
+    x[0, 0] = torch.nan
+    loss, _ = pkg().balance_loss(x.to(DEV), ids.to(DEV), torch.tensor([0, 1, 40], dtype=torch.int32, device=DEV), 1.0, score)
+    assert loss[0].isnan() and loss[1].isfinite()
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_gradient_against_differences(gpu_available, score):
+    """Central differences of the float64 loss with the kernel's gradient: the
+    step 1e-4 leaves an error of 1e-8 of the third derivative's size."""
+    x, ids, off, grad = _inputs(6, 16, 2, 2, torch.float32, 6)
+    xd = x.to(DEV).requires_grad_(True)
+    loss, _ = pkg().balance_loss(xd, ids.to(DEV), off.to(DEV), 1.0, score)
+    dx, = torch.autograd.grad(loss, xd, grad.to(DEV))
+    for t, j in ((0, 3), (2, 15), (5, 0), (4, 8)):
+        d = []
+        for h in (-1e-4, 1e-4):
+            y = x.double()
+            y[t, j] += h
+            d.append((R.balance(y, ids, off, 1.0, score)[0] * grad.double()).sum())
+        assert abs(float((d[1] - d[0]) / 2e-4) - float(dx[t, j])) < 2e-6
+
+
+def test_empty_repeat_graph_and_backward_twice(gpu_available):
+    m = pkg()
+    e = torch.empty(0, 16, device=DEV, requires_grad=True)
+    loss, counts = m.balance_loss(e, torch.empty(0, 2, dtype=torch.int32, device=DEV),
+                                  torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert (loss == 0).all() and (counts == 0).all()
+    g, = torch.autograd.grad(loss.sum(), e)
+    assert g.shape == (0, 16)
+    x, ids, off, grad = _inputs(500, 256, 8, 6, torch.float32, 8)
+    xd, idd, offd, gd = x.to(DEV).requires_grad_(True), ids.to(DEV), off.to(DEV), grad.to(DEV)
+    loss, _ = m.balance_loss(xd, idd, offd)
+    a, = torch.autograd.grad(loss, xd, gd, retain_graph=True)
+    b, = torch.autograd.grad(loss, xd, gd)
+    assert torch.equal(a, b)
+    loss2, _ = m.balance_loss(xd.detach(), idd, offd)
+    assert torch.equal(loss, loss2) and not loss2.requires_grad
+    graph = torch.cuda.CUDAGraph()
+    xs = xd.detach().clone()
+    with torch.cuda.graph(graph):
+        lg, cg = m.balance_loss(xs, idd, offd)
+    xs.copy_(xd.detach() * 0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, n, _ = R.balance(x * 0.5, ids, off, 1e-4, "sigmoid")
+    torch.testing.assert_close(lg.cpu().double(), want, rtol=2.0 ** -16, atol=0)
+    assert torch.equal(cg.cpu().long(), n)
+
+
+def test_refusals(gpu_available):
+    m = pkg()
+    x = torch.zeros(8, 16, device=DEV)
+    ids = torch.zeros(8, 2, dtype=torch.int32, device=DEV)
+    for call in (lambda: m.balance_loss(x, ids.long()), lambda: m.balance_loss(x, ids[:4]), lambda: m.balance_loss(x.int(), ids),
+                 lambda: m.balance_loss(x.t(), ids), lambda: m.balance_loss(x[0], ids), lambda: m.balance_loss(x, ids, score_func="relu"),
+                 lambda: m.balance_loss(x, ids, torch.zeros(3, device=DEV)), lambda: m.balance_loss(x, ids, torch.zeros(3, dtype=torch.int32)),
+                 lambda: m.balance_loss(torch.zeros(8, 1025, device=DEV), ids),
+                 lambda: m.balance_loss(x, torch.zeros(8, 17, dtype=torch.int32, device=DEV)),
+                 lambda: m.balance_loss(x, ids, torch.zeros(1, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            call()

@@ -1,0 +1,389 @@
+"""GPU: microscaled quantisation, residual + RMSNorm + quantisation and the
+products, against plain CPU implementations (tests/mx_reference.py)."""
+import pytest
+import torch
+
+import mx_reference as R
+from conftest import pkg
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+FMTS = list(R.BLOCK)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _hidden(rows, cols, dtype, seed):
+    """Values over many binades, some zeros, a zero block, and (16-bit types
+    apart) tiny and large ones."""
+    g = _gen(seed)
+    x = torch.randn(rows, cols, generator=g) * 2.0 ** torch.randint(-6, 7, (rows, cols // 32), generator=g).repeat_interleave(32, 1)
+    x[torch.rand(rows, cols, generator=g) < 0.05] = 0.0
+    x[0, :32] = 0.0
+    x[-1, -32:] = torch.tensor([6.0, 5.0, 3.5, 2.5, 1.75, 1.25, 0.75, 0.25]).repeat(4)  # ties of e2m1 at scale 1
+    if rows > 2:
+        x[1] *= 2.0 ** -13
+        x[2, :16] = -0.0
+    return x.to(dtype)
+
+
+def _same(got, want):
+    """Equal bytes (NaN scales included)."""
+    assert torch.equal(got.cpu().view(torch.uint8), want.view(torch.uint8))
+
+
+def _quantised(fmt, q, s, x, g=None):
+    wq, ws = R.quantize(x, fmt, g)
+    _same(s, ws)
+    if fmt == "mxfp8":
+        _same(q, wq)
+    else:
+        _same(q, R.pack(wq))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows,cols", [(1, 32), (3, 96), (17, 7168), (1000, 64)])
+def test_quantize_bit_exact(gpu_available, fmt, dtype, rows, cols):
+    x = _hidden(rows, cols, R.DTYPES[dtype], rows + cols)
+    q, s = pkg().quantize_mx(x.to(DEV), fmt)
+    _quantised(fmt, q, s, x)
+
+
+@pytest.mark.parametrize("g", [1e-3, 0.37, 3.0, 1e-30, 1e25])
+def test_quantize_global_scale(gpu_available, g):
+    x = _hidden(9, 256, torch.float32, 5)
+    gs = torch.tensor([g])
+    q, s = pkg().quantize_mx(x.to(DEV), "nvfp4", gs.to(DEV))
+    _quantised("nvfp4", q, s, x, gs)
+    y = pkg().dequantize_mx(q, s, "nvfp4", gs.to(DEV), torch.float32)
+    v = (R.values(q.cpu(), s.cpu(), "nvfp4").float() * gs).float()  # (value * scale) exact, one rounding
+    torch.testing.assert_close(y.cpu(), v, rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_extreme_and_non_finite(gpu_available, fmt):
+    x = torch.randn(6, 128, generator=_gen(2))
+    x[0, 5] = float("inf")
+    x[1, 40] = float("nan")
+    x[2, 64:96] = 3.4e38
+    x[3, :32] = 1e-45
+    x[4, 32:64] = 1.2e-38
+    x[5, 0] = -float("inf")
+    q, s = pkg().quantize_mx(x.to(DEV), fmt)
+    _quantised(fmt, q, s, x)
+    y = pkg().dequantize_mx(q, s, fmt, dtype=torch.float32).cpu()
+    v = R.values(q.cpu(), s.cpu(), fmt).float()
+    torch.testing.assert_close(y, v, rtol=0, atol=0, equal_nan=True)
+    blk = R.BLOCK[fmt]
+    assert y[0, :blk].isnan().all() and y[1, 32:32 + blk].isnan().all() and y[2].isfinite().all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+def test_dequantize_rounds_once(gpu_available, fmt, dtype):
+    q, s = R.random_packed(_gen(3), (), 37, 160, fmt)
+    y = pkg().dequantize_mx(q.to(DEV), s.to(DEV), fmt, dtype=R.DTYPES[dtype])
+    assert torch.equal(y.cpu(), R.values(q, s, fmt).to(R.DTYPES[dtype]))
+
+
+def test_quantize_strides_outputs_and_empty(gpu_available):
+    m = pkg()
+    big = torch.randn(12, 512, generator=_gen(4)).to(torch.bfloat16)
+    view = big.to(DEV)[1::2, 64:320]
+    q, s = m.quantize_mx(view, "mxfp4")
+    _quantised("mxfp4", q, s, big[1::2, 64:320])
+    out, sc = torch.empty_like(q), torch.empty_like(s)
+    a, b = m.quantize_mx(view, "mxfp4", None, out, sc)
+    assert a is out and b is sc and torch.equal(out, q)
+    back = torch.full((6, 512), 7.0, dtype=torch.float16, device=DEV)
+    m.dequantize_mx(q, s, "mxfp4", out=back[:, 128:384])
+    assert (back[:, :128] == 7).all() and (back[:, 384:] == 7).all()
+    assert torch.equal(back[:, 128:384].cpu(), R.values(q.cpu(), s.cpu(), "mxfp4").half())
+    e = torch.empty(0, 64, device=DEV)
+    for fmt in FMTS:
+        q0, s0 = m.quantize_mx(e, fmt)
+        assert q0.shape[0] == 0 and m.dequantize_mx(q0, s0, fmt).shape == (0, 64)
+        assert m.add_rmsnorm_quantize_mx(e, e.clone(), None, fmt=fmt)[0].shape[0] == 0
+
+
+def test_refusals_on_the_device(gpu_available):
+    m = pkg()
+    x = torch.zeros(4, 64, device=DEV, dtype=torch.bfloat16)
+    q, s = m.quantize_mx(x, "nvfp4")
+    bad = [lambda: m.quantize_mx(x[:, :40], "mxfp4"), lambda: m.quantize_mx(x.t(), "mxfp4"),
+           lambda: m.quantize_mx(x.long(), "mxfp4"), lambda: m.quantize_mx(x, "mxfp8", torch.ones(1, device=DEV)),
+           lambda: m.quantize_mx(x, "nvfp4", torch.ones(1)), lambda: m.quantize_mx(x, "nvfp4", torch.ones(2, device=DEV)),
+           lambda: m.quantize_mx(x.view(2, 2, 64)), lambda: m.quantize_mx(x, "nvfp4", out=q[:2]),
+           lambda: m.quantize_mx(x[:, 4:36]), lambda: m.dequantize_mx(q, s, "mxfp4"), lambda: m.dequantize_mx(q, s[:2]),
+           lambda: m.add_rmsnorm_quantize_mx(x, x.float()), lambda: m.add_rmsnorm_quantize_mx(x, None, x[0].float()),
+           lambda: m.add_rmsnorm_quantize_mx(x, eps=-1.0), lambda: m.add_rmsnorm_quantize_mx(x, x[:2]),
+           lambda: m.matmul_mx(q, s, q, s, "mxfp8"), lambda: m.matmul_mx(q, s, q[:, :16].contiguous(), s[:, :2].contiguous()),
+           lambda: m.matmul_mx(q, s, q, s, out=torch.empty(4, 5, device=DEV)),
+           lambda: m.matmul_mx(q, s, q, s, out=torch.empty(4, 4, device=DEV).t()[:, :4].long()),
+           lambda: m.matmul_mx(q, s, q, s, out_dtype=torch.int32),
+           lambda: m.matmul_mx(q, s, q, s, alpha=torch.ones(1)),
+           lambda: m.experts_matmul_mx(q, s, q[None], s[None], torch.zeros(2, device=DEV)),
+           lambda: m.experts_matmul_mx(q, s, q[None], s[None], torch.zeros(3, device=DEV, dtype=torch.int32)),
+           lambda: m.experts_matmul_mx(q, s, q, s, torch.zeros(2, device=DEV, dtype=torch.int32))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+# --------------------------------------------------------------------------
+# residual + RMSNorm + quantisation
+# --------------------------------------------------------------------------
+def _check_rows(fmt, q, s, y):
+    """Packed rows against float64 values y: within half a step of the format
+    at the scale that came back, and that scale the one y asks for (or its
+    neighbour where y's largest value is within the float32 error of a
+    border). The float32 steps before quantisation: a sum of `cols` squares
+    (<= 32 + 5 + 32 roundings), mean, add, root, reciprocal, two products:
+    under 80 half-steps of 2^-24 each, i.e. 2^-17 relative."""
+    err = 2.0 ** -17
+    y = y.cpu()
+    q, s = q.cpu(), s.cpu()
+    lo, hi = [R.quantize((y * (1 + d)).float(), fmt)[1] for d in (-err, err)]
+    sv, lo, hi = (R.scale_values(v) for v in (s, lo, hi))
+    assert ((sv >= lo) & (sv <= hi)).all()
+    sv = sv.repeat_interleave(R.BLOCK[fmt], 1)
+    v = R.values(q, s, fmt)
+    t = torch.where(sv > 0, y.abs() / sv, 0.0)
+    if fmt == "mxfp8":
+        step = torch.maximum(2.0 ** (torch.floor(torch.log2(t.clamp(min=2.0 ** -6))) - 3), torch.full_like(t, 2.0 ** -9))
+        half = step / 2 + (t - 448).clamp(min=0)
+    else:
+        half = torch.where(t < 2, 0.25, torch.where(t < 4, 0.5, 1.0)) + (t - 6).clamp(min=0)
+    assert ((v - y).abs() <= half * sv + err * y.abs() + 1e-300).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows,cols", [(1, 32), (5, 96), (9, 1024), (3, 1056), (33, 7168), (2, 8224), (2, 32768)])
+def test_norm(gpu_available, fmt, dtype, rows, cols):
+    dt = R.DTYPES[dtype]
+    g = _gen(rows + cols)
+    x, res = (torch.randn(rows, cols, generator=g).to(dt) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(cols, generator=g)).to(dt)
+    res_d = res.to(DEV)
+    q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), res_d, w.to(DEV), 1e-5, fmt)
+    h = (x.float() + res.float()).to(dt)
+    assert torch.equal(res_d.cpu(), h)
+    h = h.double()
+    y = h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-5) * w.double()
+    _check_rows(fmt, q, s, y)
+
+
+def test_norm_without_residual_or_weight(gpu_available):
+    m = pkg()
+    x = torch.randn(7, 256, generator=_gen(8)).to(torch.bfloat16)
+    q, s = m.add_rmsnorm_quantize_mx(x.to(DEV), None, None, fmt="mxfp4")
+    _quantised("mxfp4", q, s, x)                       # y = h = x
+    w = torch.ones(256, dtype=torch.bfloat16)
+    xd = x.to(DEV)
+    q, s = m.add_rmsnorm_quantize_mx(xd, None, w.to(DEV), 1e-6, "mxfp8")
+    assert torch.equal(xd.cpu(), x)
+    h = x.double()
+    _check_rows("mxfp8", q, s, h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-6))
+
+
+def test_norm_strides_global_scale_zero_row_and_nan_row(gpu_available):
+    m = pkg()
+    g = _gen(9)
+    big = torch.randn(10, 640, generator=g)
+    big[2] = 0.0
+    big[4, 300] = float("nan")
+    x = big.to(DEV)[::2, 128:512]
+    res = torch.zeros(5, 400, device=DEV)
+    res[:, 384:] = 3.0
+    w = torch.rand(384, generator=g) + 0.5
+    gs = torch.tensor([0.01])
+    q, s = m.add_rmsnorm_quantize_mx(x, res[:, :384], w.to(DEV), 1e-6, "nvfp4", gs.to(DEV))
+    assert (res[:, 384:] == 3).all()
+    h = big[::2, 128:512].double()
+    y = h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-6) * w.double()
+    deq = m.dequantize_mx(q, s, "nvfp4", gs.to(DEV), torch.float32).cpu().double()
+    assert (deq[1] == 0).all() and deq[2].isnan().all()
+    ok = [0, 3, 4]
+    # half a step of e2m1 (1/4 of the value at most, 1/12 of the block's largest) and the scale's 2^-4
+    bound = y.abs() * (0.25 + 2.0 ** -4) + y.abs().view(5, -1, 16).amax(-1).repeat_interleave(16, 1) / 12
+    assert ((deq - y).abs()[ok] <= bound[ok] * 1.01).all()
+
+
+# --------------------------------------------------------------------------
+# products
+# --------------------------------------------------------------------------
+def _product_ok(got, a, b, alpha, dt, note=""):
+    """Against float64. The tensor core adds 32 or 64 exact products at a time
+    to a float32 sum. Counted: one float32 step (2^-23) of the sum of
+    magnitudes for every 32 values of K and 8 more for the alignment inside a
+    step, the split's additions and alpha; then half a step of the output's type."""
+    ref, mag = a @ b.t(), a.abs() @ b.abs().t()
+    tol = (a.shape[1] / 32 + 8) * 2.0 ** -23 * mag * abs(alpha) + torch.finfo(dt).eps / 2 * (ref * alpha).abs() * 1.01
+    bad = (got.cpu().double() - ref * alpha).abs() > tol + 1e-30
+    assert not bad.any(), f"{note}: {int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}"
+
+
+# rows x weight rows x width: one token, tile borders of both, K ends inside a
+# stage and inside a scale word, K splits of 2..8, several tiles a CTA
+SHAPES = [(1, 128, 256), (1, 1, 32), (1, 4096, 7168), (8, 130, 96), (16, 128, 512), (17, 300, 480), (33, 257, 2048), (64, 64, 1024),
+          (65, 129, 736), (127, 512, 288), (200, 384, 4096), (256, 256, 256), (257, 128, 1184), (1000, 7168, 160), (700, 6000, 224)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_matmul(gpu_available, fmt, m, n, k):
+    g = _gen(m + n + k)
+    a, sa = R.random_packed(g, (), m, k, fmt)
+    b, sb = R.random_packed(g, (), n, k, fmt)
+    out = pkg().matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), fmt, out_dtype=torch.float32)
+    assert pkg().device_status() == 0
+    _product_ok(out, R.values(a, sa, fmt), R.values(b, sb, fmt), 1.0, torch.float32, f"{fmt} {m} {n} {k}")
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+def test_matmul_types_alpha_and_strided_output(gpu_available, dtype):
+    dt = R.DTYPES[dtype]
+    g = _gen(12)
+    a, sa = R.random_packed(g, (), 70, 320, "nvfp4", 1)
+    b, sb = R.random_packed(g, (), 201, 320, "nvfp4", 1)
+    out = torch.full((72, 211), 9.0, dtype=dt, device=DEV)
+    al = torch.tensor([0.0173])
+    got = pkg().matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), "nvfp4", al.to(DEV), out=out[1:71, 3:204])
+    assert got.data_ptr() == out[1:, 3:].data_ptr()
+    _product_ok(got, R.values(a, sa, "nvfp4"), R.values(b, sb, "nvfp4"), float(al), dt)
+    assert (out[0] == 9).all() and (out[71] == 9).all() and (out[:, :3] == 9).all() and (out[:, 204:] == 9).all()
+
+
+def test_matmul_nan_scale_stays_in_its_row(gpu_available):
+    g = _gen(13)
+    a, sa = R.random_packed(g, (), 40, 512, "mxfp4")
+    b, sb = R.random_packed(g, (), 140, 512, "mxfp4")
+    sa.view(torch.uint8)[7, 3] = 255
+    sb.view(torch.uint8)[131, 9] = 255
+    out = pkg().matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), "mxfp4", out_dtype=torch.float32).cpu()
+    nan = torch.zeros(40, 140, dtype=torch.bool)
+    nan[7] = nan[:, 131] = True
+    assert torch.equal(out.isnan(), nan)
+
+
+def test_matmul_empty(gpu_available):
+    m = pkg()
+    b, sb = (t.to(DEV) for t in R.random_packed(_gen(1), (), 8, 64, "nvfp4"))
+    out = m.matmul_mx(b[:0], sb[:0], b, sb)
+    assert out.shape == (0, 8)
+    e = m.experts_matmul_mx(b[:0], sb[:0], b[None], sb[None], torch.zeros(2, dtype=torch.int32, device=DEV))
+    assert e.shape == (0, 8)
+
+
+def _runs(counts, first=0):
+    off = torch.tensor([first] + list(counts)).cumsum(0).int()
+    return off, int(off[-1])
+
+
+EXPERTS = [([1], 128, 256), ([0, 0, 1, 0], 256, 7168), ([3, 0, 17, 1, 16], 130, 96), ([40, 0, 0, 250, 5, 129], 300, 480),
+           ([1] * 40, 64, 512), ([2] * 33 + [0] * 70 + [300], 128, 736), ([500, 0, 1], 200, 2048), ([0, 0], 128, 64)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("counts,n,k", EXPERTS)
+def test_experts_matmul(gpu_available, fmt, counts, n, k):
+    """Ragged runs, empty ones among them, rows before and behind them left as they were."""
+    off, end = _runs(counts, 2)
+    rows, e = end + 3, len(counts)
+    g = _gen(sum(counts) + n + k)
+    a, sa = R.random_packed(g, (), rows, k, fmt)
+    b, sb = R.random_packed(g, (e,), n, k, fmt)
+    al = torch.rand(e, generator=g) + 0.5
+    out = torch.full((rows, n), 5.0, device=DEV)
+    pkg().experts_matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), off.to(DEV), fmt, al.to(DEV), out=out)
+    assert pkg().device_status() == 0
+    assert (out[:2] == 5).all() and (out[end:] == 5).all()
+    av = R.values(a, sa, fmt)
+    for i, c in enumerate(counts):
+        if c:
+            lo = int(off[i])
+            _product_ok(out[lo:lo + c], av[lo:lo + c], R.values(b[i], sb[i], fmt), float(al[i]), torch.float32, f"expert {i}")
+
+
+def test_experts_matmul_without_out_is_zero_outside(gpu_available):
+    g = _gen(21)
+    a, sa = (t.to(DEV) for t in R.random_packed(g, (), 9, 64, "nvfp4"))
+    b, sb = (t.to(DEV) for t in R.random_packed(g, (2,), 8, 64, "nvfp4"))
+    out = pkg().experts_matmul_mx(a, sa, b, sb, torch.tensor([2, 4, 4], dtype=torch.int32, device=DEV))
+    assert out.dtype == torch.bfloat16 and (out[:2] == 0).all() and (out[4:] == 0).all() and (out[2:4] != 0).any()
+
+
+def test_products_are_repeatable_on_streams_and_in_graphs(gpu_available):
+    """The same bits again, from two streams at once and from a replayed graph
+    whose inputs have changed."""
+    m = pkg()
+    g = _gen(31)
+    a, sa = (t.to(DEV) for t in R.random_packed(g, (), 24, 4096, "nvfp4"))
+    b, sb = (t.to(DEV) for t in R.random_packed(g, (), 512, 4096, "nvfp4"))
+    a2, sa2 = (t.to(DEV) for t in R.random_packed(g, (), 24, 4096, "nvfp4"))
+    first, second = m.matmul_mx(a, sa, b, sb), m.matmul_mx(a2, sa2, b, sb)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(first) for _ in range(2)]
+    for _ in range(10):
+        for st, o, (x, sx) in zip(streams, outs, ((a, sa), (a2, sa2))):
+            with torch.cuda.stream(st):
+                m.matmul_mx(x, sx, b, sb, out=o)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], first) and torch.equal(outs[1], second)
+    x, sx, o = a.clone(), sa.clone(), torch.empty_like(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m.matmul_mx(x, sx, b, sb, out=o)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, first)
+    x.copy_(a2)
+    sx.copy_(sa2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, second) and m.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_expert_mlp_after_routing(gpu_available, fmt):
+    """The operators as a layer uses them: residual + norm + quantise, route,
+    rows sorted by expert, gate and up products, SwiGLU, quantise, down
+    products, weighted sum; against float64 of the same quantised values."""
+    m = pkg()
+    T, H, I, E = 24, 512, 256, 32
+    g = _gen(41)
+    x, res = (torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(H, generator=g)).to(torch.bfloat16).to(DEV)
+    logits = torch.randn(T, 256, generator=g).to(DEV)
+    bias = torch.zeros(256, dtype=torch.bfloat16, device=DEV)
+    ids, wts, _ = m.route(logits, bias, 0, E, 2.5)
+    loss, counts = m.balance_loss(logits, ids)
+    flat = ids.flatten()
+    local = flat < E
+    order = torch.argsort(torch.where(local, flat, E), stable=True)[: int(local.sum())]
+    tok, exp = order // 8, flat[order]
+    off = torch.cat((counts.new_zeros(1, 1), counts[:, :E].cumsum(1)), 1).flatten().int()
+    assert int(off[-1]) == order.numel()
+    q, s = m.add_rmsnorm_quantize_mx(x, res, w, 1e-6, fmt)
+    w13, s13 = (t.to(DEV) for t in R.random_packed(g, (E,), 2 * I, H, fmt))
+    w2, s2 = (t.to(DEV) for t in R.random_packed(g, (E,), H, I, fmt))
+    qa, sa = q[tok].contiguous(), s.view(torch.uint8)[tok].contiguous().view(s.dtype)
+    h = m.experts_matmul_mx(qa, sa, w13, s13, off, fmt, out_dtype=torch.float32)
+    act = h[:, :I] * (h[:, I:] * 2.0 ** -8).sigmoid()
+    qi, si = m.quantize_mx(act, fmt)
+    y = m.experts_matmul_mx(qi, si, w2, s2, off, fmt, out_dtype=torch.float32)
+    out = torch.zeros(T, H, device=DEV).index_add_(0, tok, y * wts.flatten()[order][:, None])
+    assert m.device_status() == 0
+    av, iv = R.values(qa.cpu(), sa.cpu(), fmt), R.values(qi.cpu(), si.cpu(), fmt)
+    for e in exp.unique().tolist():
+        r = (exp == e).nonzero().flatten().cpu()
+        _product_ok(h[r], av[r], R.values(w13[e].cpu(), s13[e].cpu(), fmt), 1.0, torch.float32)
+        _product_ok(y[r], iv[r], R.values(w2[e].cpu(), s2[e].cpu(), fmt), 1.0, torch.float32)
+    assert out.isfinite().all() and (out.abs().sum(1) > 0).any()
