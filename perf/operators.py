@@ -121,7 +121,7 @@ def _quantize(x, fmt, g=None):
     if fmt == "mxfp8":
         return t.clamp(-448.0, 448.0).to(torch.float8_e4m3fn), scale
     c = _e2m1_code(t)
-    return c[:, 0::2] | (c[:, 1::2] << 4), scale
+    return (c[:, 0::2] | (c[:, 1::2] << 4)).to(torch.uint8), scale
 
 
 def _scale_values(scale):
