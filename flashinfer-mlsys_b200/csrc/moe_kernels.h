@@ -203,15 +203,17 @@ struct MxGemmCall {
   int fmt;
 };
 struct MxPlan {
-  int tn;     // tokens of a tile (the token map's box rows)
-  int nt;     // kernel variant: tile room
-  int split;  // cluster size along K
+  int tn;        // tokens of a tile
+  int box_rows;  // rows of the token map's boxes
+  int nt;        // kernel variant: tile room
+  bool pair;     // a pair of CTAs shares a tile of 256 weight rows
+  int split;     // cluster size along K
   int grid;
 };
 constexpr int kMxGemmMaxExperts = 512;
 int mx_gemm_stages(int64_t K, int fmt);
 MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs);
-// map_w: weights [experts][N][K bytes], boxes of 128 rows x 128 bytes; map_a: tokens [rows][K bytes], boxes of plan.tn rows
+// map_w: weights [experts][N][K bytes], boxes of 128 rows x 128 bytes; map_a: tokens [rows][K bytes], boxes of plan.box_rows rows
 cudaError_t launch_mx_gemm(const CUtensorMap& map_w, const CUtensorMap& map_a, const MxGemmCall& c, const MxPlan& pl,
                            cudaStream_t s);
 cudaError_t mx_take_status(unsigned* v);  // reads and clears the product's status word (synchronous)

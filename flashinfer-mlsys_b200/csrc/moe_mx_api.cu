@@ -70,7 +70,7 @@ int matmul(const void* a, const void* a_scale, const void* b, const void* b_scal
   const MxPlan pl = mx_gemm_plan(M, N, static_cast<int>(experts), mx_gemm_stages(K, fmt), off != nullptr);
   CUtensorMap mw, ma;
   if (!encode_map_3d(&mw, b, row_bytes, static_cast<uint64_t>(N), static_cast<uint64_t>(experts), 128) ||
-      !encode_map_3d(&ma, a, row_bytes, static_cast<uint64_t>(M), 1, static_cast<uint32_t>(pl.tn)))
+      !encode_map_3d(&ma, a, row_bytes, static_cast<uint64_t>(M), 1, static_cast<uint32_t>(pl.box_rows)))
     return MOE_ERR_CUDA;
   MxGemmCall c{};
   c.a_scale = a_scale;

@@ -15,10 +15,10 @@
 //                token tile per stage (256 4-bit or 128 8-bit values)
 //   warp 1       TMEM owner and MMA issuer: copies the stage's scales to TMEM
 //                (tcgen05.cp) and issues four K slices of 32 bytes
-//   warps 2-5    scale loaders, a stage each in turn. Scales are stored row by
+//   warps 2-5    scale loaders, four stages at a time. Scales are stored row by
 //                row; the tensor core wants, for 128 rows, word w of row r at
-//                lane r % 32, column r / 32. A lane loads the words of rows
-//                l, l + 32, l + 64, l + 96 and stores them transposed.
+//                lane r % 32, column r / 32: a lane loads the words of rows
+//                r, r + 32, r + 64, r + 96 and stores them transposed.
 //   warps 6-13   epilogue: TMEM -> registers -> global, two warps a lane quarter
 // TMEM (512 columns): two slots of scales at the top and two accumulators of
 // the tile's width below, which overlap in their middle when two do not fit;
@@ -45,20 +45,21 @@ constexpr uint64_t kMxWaitNs = 2000000000ull;  // 2 s: only reached if something
 
 __device__ unsigned g_mx_status;  // kErrTimeout if a bounded wait gave up
 
-template <int kFmt, int kNT>
+template <int kFmt, int kNT, bool kPair>
 struct MxCfg {
   static constexpr int kW = kFmt == kFmtNvfp4 ? 4 : (kFmt == kFmtMxfp4 ? 2 : 1);  // scale words of a row and stage
   static constexpr int kChunks = kNT > 128 ? 2 : 1;                               // 128-token groups of scales
   static constexpr int kTileBytes = kMxTileN * kMxStageK;
-  static constexpr int kStageBytes = kTileBytes + kNT * kMxStageK;
+  static constexpr int kStageBytes = kTileBytes + (kPair ? kNT / 2 : kNT) * kMxStageK;  // a pair halves the tokens
   static constexpr int kSfBytes = kW * 512 * (1 + kChunks);
-  static constexpr int kStages = kNT > 128 ? 4 : (kNT > 64 ? 6 : (kNT > 32 ? 6 : 8));
+  static constexpr int kStages = kPair ? 5 : (kNT > 64 ? 5 : (kNT > 32 ? 6 : 8));
+  static constexpr int kGroupBytes = 4 * kSfBytes;  // scales of four stages
   static constexpr int kSfCols = kW * 4 * (1 + kChunks);  // TMEM columns of one slot
   static constexpr int kAccCols = (512 - 2 * kSfCols) & ~31;
-  static constexpr int kOwnPart = kNT <= 64;              // room for the split's partial sums beside the ring
+  static constexpr bool kOwnPart = kNT <= 64;             // room for the split's partial sums beside the ring
   static constexpr int kPartBytes = kNT * kMxTileN * 4;
   static constexpr size_t kSmem =
-      1024 + (size_t)kStages * (kStageBytes + kSfBytes) + (kOwnPart ? kPartBytes : 0);
+      1024 + (size_t)kStages * kStageBytes + 2 * kGroupBytes + (kOwnPart ? kPartBytes : 0);
   static_assert(kOwnPart || kPartBytes <= kStages * kStageBytes, "partial sums reuse the ring");
 };
 
@@ -78,7 +79,7 @@ struct MxGemmArgs {
 };
 
 struct __align__(16) MxCtl {
-  uint64_t full[8], empty[8], tfull[2], acc_free, part_ready, part_free, mma_done;
+  uint64_t full[8], empty[8], sf_full[2], sf_empty[2], tfull[2], acc_free, part_ready, part_free, mma_done;
   uint32_t tmem_base;
   int abort_flag;
   int start[kMxMaxExperts + 1];   // first row of each run
@@ -90,10 +91,10 @@ struct MxUnit {
   int e, n0, row0, cnt;
 };
 
-__device__ __forceinline__ MxUnit mx_unit(const MxCtl* c, const MxGemmArgs& p, int u, int ntn) {
+__device__ __forceinline__ MxUnit mx_unit(const MxCtl* c, const MxGemmArgs& p, int u, int ntn, int tile_rows) {
   MxUnit x;
   const int g = u / ntn;
-  x.n0 = (u - g * ntn) * kMxTileN;
+  x.n0 = (u - g * ntn) * tile_rows;
   int lo = 0, hi = p.E - 1;
   while (lo < hi) {  // last run whose first tile is <= g (empty runs share prefixes)
     const int mid = (lo + hi + 1) >> 1;
@@ -121,52 +122,94 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// The same into this CTA's shared memory, counted on the barrier at `bar` (a
+// cluster address): both CTAs of a pair count on the first one's.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
 // 32 rows x 16 bytes of shared memory (rows 16 bytes apart) to 4 TMEM columns
 // of lanes 0-31, repeated in the other three lane quarters.
+template <bool kPair>
 __device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint32_t smem_addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
   d |= static_cast<uint64_t>(128u >> 4) << 16;  // leading offset (one 16-byte column only: unused)
   d |= static_cast<uint64_t>(128u >> 4) << 32;  // 128 B between 8-row groups
   d |= static_cast<uint64_t>(1u) << 46;         // descriptor version, no swizzle
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  if constexpr (kPair)  // in both CTAs, each from its own shared memory
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
-// Instruction descriptor of the block-scaled kinds, A and B K-major, M = 128:
+// Instruction descriptor of the block-scaled kinds, A and B K-major, M = 128 (256 for a pair):
 // scale id of B in [4,6), type of A in [7,10) and of B in [10,13) (e2m1 = 1 in
 // the 4-bit kinds, e4m3 = 0 in mxf8f6f4), N >> 3 in [17,23), scale type bit 23
 // (0 e4m3, 1 e8m0), M >> 7 in [27,29), scale id of A in [29,31). The scale id
 // is the byte of the 32-bit scale word that holds the K slice's first scale.
-template <int kFmt>
+template <int kFmt, bool kPair>
 __device__ __forceinline__ uint32_t mx_idesc(int n, uint32_t id) {
   const uint32_t type = kFmt == kFmtMxfp8 ? 0u : 1u;
   const uint32_t scale = kFmt == kFmtNvfp4 ? 0u : 1u;
-  return (id << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (scale << 23) | (1u << 27) |
-         (id << 29);
+  return (id << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (scale << 23) |
+         ((kPair ? 2u : 1u) << 27) | (id << 29);
 }
 
-template <int kFmt>
+#define MX_MMA(GROUP, KIND)                                                                              \
+  asm volatile(                                                                                         \
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                  \
+      "tcgen05.mma.cta_group::" GROUP "." KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),       \
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)                                            \
+      : "memory")
+template <int kFmt, bool kPair>
 __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                        uint32_t acc) {
   if constexpr (kFmt == kFmtNvfp4) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
-        : "memory");
+    if constexpr (kPair) MX_MMA("2", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+    else MX_MMA("1", "kind::mxf4nvf4.block_scale.scale_vec::4X");
   } else if constexpr (kFmt == kFmtMxfp4) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
-        : "memory");
+    if constexpr (kPair) MX_MMA("2", "kind::mxf4.block_scale.scale_vec::2X");
+    else MX_MMA("1", "kind::mxf4.block_scale.scale_vec::2X");
   } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
-        : "memory");
+    if constexpr (kPair) MX_MMA("2", "kind::mxf8f6f4.block_scale.scale_vec::1X");
+    else MX_MMA("1", "kind::mxf8f6f4.block_scale.scale_vec::1X");
   }
+}
+#undef MX_MMA
+
+// Arrive on `bar` (of both CTAs of a pair) once this thread's earlier MMAs and copies are done.
+template <bool kPair>
+__device__ __forceinline__ void mx_commit(uint64_t* bar) {
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(
+            smem_u32(bar))
+        : "memory");
+  else
+    mma_commit(bar);
+}
+template <bool kPair>
+__device__ __forceinline__ void mx_tmem_alloc(uint32_t* dst) {
+  if constexpr (kPair) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, 512);
+    tmem_relinquish();
+  }
+}
+template <bool kPair>
+__device__ __forceinline__ void mx_tmem_dealloc(uint32_t taddr) {
+  if constexpr (kPair)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+  else
+    tmem_dealloc(taddr, 512);
 }
 
 // ---- cluster helpers --------------------------------------------------------
@@ -203,6 +246,22 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "memory");
   return v;
 }
+// A barrier of the first CTA of a pair, on which both arrive; otherwise this CTA's own.
+template <bool kPair>
+__device__ __forceinline__ void mx_arrive(uint64_t* bar) {
+  if constexpr (kPair)
+    cluster_arrive_remote(cluster_map(smem_u32(bar), 0));
+  else
+    mbar_arrive(bar);
+}
+template <bool kPair>
+__device__ __forceinline__ bool mx_wait(uint64_t* bar, uint32_t parity) {
+  if constexpr (kPair)
+    return cluster_wait_bounded(bar, parity, kMxWaitNs);
+  else
+    return mbar_wait_bounded(bar, parity, kMxWaitNs);
+}
+
 __device__ __forceinline__ void epi_bar_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 static_assert(kMxEpiWarps * 32 == 256, "epi_bar_sync counts the epilogue's threads");
 
@@ -216,76 +275,82 @@ __device__ __forceinline__ void mx_out_store(const MxGemmArgs& p, int64_t row, i
     static_cast<float*>(p.out)[i] = v;
 }
 
-// ---- scales of up to 128 rows into the tensor core's order --------------------
-// `base`: the first row's scales at the stage's first scale; `left`: scales of
-// a row from there on. mode 2: rows are whole words, vector loads; 1: words;
-// 0: bytes (any row length).
+// The scale words of one row and stage: `left` scales remain in the row from
+// `s` on (none: zeros). mode 2: rows are whole stages, one vector load; 1:
+// words; 0: bytes (any row length).
 template <int kW>
-__device__ __forceinline__ void mx_sf_load(const uint8_t* base, int64_t nsc, int rows, int left, int mode, int lane,
-                                           uint32_t (&w)[4][kW]) {
+__device__ __forceinline__ void mx_sf_load(const uint8_t* s, int left, int mode, uint32_t (&w)[kW]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = lane + 32 * j;
-#pragma unroll
-    for (int i = 0; i < kW; ++i) w[j][i] = 0;
-    if (r >= rows) continue;
-    const uint8_t* s = base + r * nsc;
-    if (mode == 2) {
-      if constexpr (kW == 4) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
-        w[j][0] = v.x, w[j][1] = v.y, w[j][2] = v.z, w[j][3] = v.w;
-      } else if constexpr (kW == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-        w[j][0] = v.x, w[j][1] = v.y;
-      } else {
-        w[j][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
-      }
-    } else if (mode == 1) {
-#pragma unroll
-      for (int i = 0; i < kW; ++i)
-        if (4 * i < left) w[j][i] = __ldg(reinterpret_cast<const uint32_t*>(s) + i);
+  for (int i = 0; i < kW; ++i) w[i] = 0;
+  if (left <= 0) return;
+  if (mode == 2) {
+    if constexpr (kW == 4) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (kW == 2) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+      w[0] = v.x, w[1] = v.y;
     } else {
-#pragma unroll
-      for (int i = 0; i < 4 * kW; ++i)
-        if (i < left) w[j][i / 4] |= static_cast<uint32_t>(__ldg(s + i)) << (8 * (i % 4));
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
     }
+  } else if (mode == 1) {
+#pragma unroll
+    for (int i = 0; i < kW; ++i)
+      if (4 * i < left) w[i] = __ldg(reinterpret_cast<const uint32_t*>(s) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * kW; ++i)
+      if (i < left) w[i / 4] |= static_cast<uint32_t>(__ldg(s + i)) << (8 * (i % 4));
   }
 }
-template <int kW>
-__device__ __forceinline__ void mx_sf_store(uint8_t* dst, int word_stride, int lane, const uint32_t (&w)[4][kW]) {
-#pragma unroll
-  for (int i = 0; i < kW; ++i)
-    *reinterpret_cast<uint4*>(dst + i * word_stride + lane * 16) = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
+
+// A bounded wait gives up for the whole warp or for none of it.
+__device__ __forceinline__ bool all_lanes(bool ok) { return __all_sync(0xffffffffu, ok); }
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
-template <int kFmt, int kNT>
+template <int kFmt, int kNT, bool kPair>
 __global__ void __launch_bounds__(kMxGemmThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                    const MxGemmArgs p) {
-  using Cfg = MxCfg<kFmt, kNT>;
+  using Cfg = MxCfg<kFmt, kNT, kPair>;
   constexpr int kS = Cfg::kStages, kW = Cfg::kW;
   extern __shared__ uint8_t smem_raw[];
   __shared__ MxCtl ctl_;
   MxCtl* ctl = &ctl_;
   uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sfs = tiles + kS * Cfg::kStageBytes;
-  float* part = reinterpret_cast<float*>(Cfg::kOwnPart ? sfs + kS * Cfg::kSfBytes : tiles);
+  float* part = reinterpret_cast<float*>(Cfg::kOwnPart ? sfs + 2 * Cfg::kGroupBytes : tiles);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int ntn = (p.N + kMxTileN - 1) / kMxTileN;
-  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
-  const int u_first = blockIdx.x / p.split, u_step = gridDim.x / p.split;
-  const int k0 = static_cast<int>((static_cast<int64_t>(p.nk) * rank) / p.split);
-  const int k1 = static_cast<int>((static_cast<int64_t>(p.nk) * (rank + 1)) / p.split);
+  // a unit is one tile of weight rows x tokens, and belongs to a cluster: a
+  // pair (256 weight rows, 128 a CTA) or `split` CTAs along K (1: no cluster)
+  const bool clustered = kPair || p.split > 1;
+  const int members = kPair ? 2 : p.split;
+  constexpr int kTileRows = kPair ? 2 * kMxTileN : kMxTileN;
+  const int ntn = (p.N + kTileRows - 1) / kTileRows;
+  const int rank = clustered ? blockIdx.x % members : 0;
+  const int u_first = blockIdx.x / members, u_step = gridDim.x / members;
+  const int k0 = kPair ? 0 : static_cast<int>((static_cast<int64_t>(p.nk) * rank) / p.split);
+  const int k1 = kPair ? p.nk : static_cast<int>((static_cast<int64_t>(p.nk) * (rank + 1)) / p.split);
+  const int my_n = kPair ? rank * kMxTileN : 0;  // first weight row of this CTA inside the tile
 
   if (tid == 0) {
     for (int s = 0; s < kS; ++s) {
-      mbar_init(&ctl->full[s], 2);   // the TMA thread and the scale warp
+      mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ctl->sf_full[b], kPair ? 2 * kMxSfWarps : kMxSfWarps);
+      mbar_init(&ctl->sf_empty[b], 1);
     }
     mbar_init(&ctl->tfull[0], 1);
     mbar_init(&ctl->tfull[1], 1);
-    mbar_init(&ctl->acc_free, kMxEpiWarps);
+    mbar_init(&ctl->acc_free, kPair ? 2 * kMxEpiWarps : kMxEpiWarps);
     mbar_init(&ctl->part_ready, p.split);
     mbar_init(&ctl->part_free, p.split);
     mbar_init(&ctl->mma_done, 1);
@@ -295,8 +360,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     prefetch_tensormap(&map_a);
   }
   if (warp == 1) {
-    tmem_alloc(&ctl->tmem_base, 512);
-    tmem_relinquish();
+    mx_tmem_alloc<kPair>(&ctl->tmem_base);
   }
   griddep_wait();
   griddep_launch_dependents();
@@ -329,7 +393,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     if (lane == 0) ctl->prefix[p.E] = base;
   }
   tc_fence_before();
-  if (p.split > 1)
+  if (clustered)
     cluster_sync_all();  // the barriers of every CTA of the cluster are set up
   else
     __syncthreads();
@@ -344,102 +408,146 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     // ======================= TMA producer =======================
     if (lane == 0) {
       uint32_t it = 0;
+      const int rows_a = kPair ? p.tn / 2 : p.tn;  // token rows of this CTA's box
       for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
-        const MxUnit x = mx_unit(ctl, p, u, ntn);
+        const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+        // the second CTA of a pair holds the second half of the columns that are issued
+        const int row_a = x.row0 + (kPair ? rank * ((x.cnt + 15) / 16 * 8) : 0);
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % kS;
           if (!mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs)) { mx_abort(ctl); break; }
           uint8_t* st = tiles + s * Cfg::kStageBytes;
-          mbar_arrive_expect_tx(&ctl->full[s], Cfg::kTileBytes + p.tn * kMxStageK);
-          tma_load_3d(st, &map_w, k * kMxStageK, x.n0, x.e, &ctl->full[s]);
-          tma_load_3d(st + Cfg::kTileBytes, &map_a, k * kMxStageK, x.row0, 0, &ctl->full[s]);
+          const uint32_t bytes = Cfg::kTileBytes + rows_a * kMxStageK;
+          if constexpr (kPair) {
+            // both CTAs' copies count on the first CTA's barrier
+            const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
+            if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * bytes);
+            tma_load_3d_pair(st, &map_w, k * kMxStageK, x.n0 + my_n, x.e, bar);
+            tma_load_3d_pair(st + Cfg::kTileBytes, &map_a, k * kMxStageK, row_a, 0, bar);
+          } else {
+            mbar_arrive_expect_tx(&ctl->full[s], bytes);
+            tma_load_3d(st, &map_w, k * kMxStageK, x.n0, x.e, &ctl->full[s]);
+            tma_load_3d(st + Cfg::kTileBytes, &map_a, k * kMxStageK, row_a, 0, &ctl->full[s]);
+          }
         }
       }
       if (mx_aborted(ctl)) {
-        // wait (bounded) for the copies this thread may still have in flight
-        for (uint32_t j = it > (uint32_t)kS ? it - kS : 0; j < it; ++j)
-          mbar_wait_bounded(&ctl->full[j % kS], (j / kS) & 1u, kMxWaitNs);
+        // wait (bounded) for the copies in flight; the second CTA of a pair,
+        // whose copies count elsewhere, gives them a millisecond
+        if (rank == 0 || !kPair) {
+          for (uint32_t j = it > (uint32_t)kS ? it - kS : 0; j < it; ++j)
+            mbar_wait_bounded(&ctl->full[j % kS], (j / kS) & 1u, kMxWaitNs);
+        } else {
+          const uint64_t t0 = global_timer_ns();
+          while (global_timer_ns() - t0 < 1000000) __nanosleep(1000);
+        }
       }
     }
   } else if (warp == 1) {
     // ======================= MMA issuer =======================
-    if (lane == 0) {
-      uint32_t it = 0, tile = 0;
+    // The whole warp walks the loop and one elected lane issues: with every
+    // operand the same in all lanes an issue costs a few cycles, where a
+    // branch on the lane cost some 70 for each (182 -> 145 us at 8192 x 7168 x 4096 nvfp4).
+    if (!kPair || rank == 0) {
+      uint32_t it = 0, tile = 0, grp = 0;
+      const bool el = elect_one();
       for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step, ++tile) {
-        const MxUnit x = mx_unit(ctl, p, u, ntn);
+        const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
         const int nmma = (x.cnt + 15) & ~15;
         const uint32_t d = acc_at[tile & 1u];
         // the tile before last has left this accumulator and the last one the columns they share
-        if (tile > 0 && !mbar_wait_bounded(&ctl->acc_free, (tile - 1) & 1u, kMxWaitNs)) { mx_abort(ctl); break; }
+        if (tile > 0 && !all_lanes(mx_wait<kPair>(&ctl->acc_free, (tile - 1) & 1u))) { mx_abort(ctl); break; }
         for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % kS;
-          // the scale slot's last readers have finished (two stages back)
-          if (it >= 2 && !mbar_wait_bounded(&ctl->empty[(it - 2) % kS], ((it - 2) / kS) & 1u, kMxWaitNs)) { mx_abort(ctl); break; }
-          if (!mbar_wait_bounded(&ctl->full[s], (it / kS) & 1u, kMxWaitNs)) { mx_abort(ctl); break; }
+          const int s = it % kS, kg = (k - k0) & 3;
+          const uint32_t gs = grp & 1u;
+          if (kg == 0 && !all_lanes(mx_wait<kPair>(&ctl->sf_full[gs], (grp >> 1) & 1u))) { mx_abort(ctl); break; }
+          // the TMEM scale slot's last readers have finished (two stages back)
+          if (it >= 2 && !all_lanes(mbar_wait_bounded(&ctl->empty[(it - 2) % kS], ((it - 2) / kS) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+          if (!all_lanes(mx_wait<kPair>(&ctl->full[s], (it / kS) & 1u))) { mx_abort(ctl); break; }
           tc_fence_after();
-          const uint32_t sf = smem_u32(sfs + s * Cfg::kSfBytes);
-          const uint32_t t_w = sf_at + (it & 1u) * Cfg::kSfCols, t_a = t_w + 4 * kW;
+          const bool group_ends = kg == 3 || k == k1 - 1;
+          if (el) {
+            const uint32_t sf = smem_u32(sfs + gs * Cfg::kGroupBytes + kg * Cfg::kSfBytes);
+            const uint32_t t_w = sf_at + (it & 1u) * Cfg::kSfCols, t_a = t_w + 4 * kW;
 #pragma unroll
-          for (int i = 0; i < kW; ++i) {
-            tmem_cp_sf(t_w + 4 * i, sf + i * 512);
+            for (int i = 0; i < kW; ++i) {
+              tmem_cp_sf<kPair>(t_w + 4 * i, sf + i * 512);
 #pragma unroll
-            for (int c = 0; c < Cfg::kChunks; ++c)
-              if (c * 128 < nmma)
-                tmem_cp_sf(t_a + (i * Cfg::kChunks + c) * 4, sf + kW * 512 + (i * Cfg::kChunks + c) * 512);
+              for (int c = 0; c < Cfg::kChunks; ++c)
+                if (c * 128 < nmma)
+                  tmem_cp_sf<kPair>(t_a + (i * Cfg::kChunks + c) * 4, sf + kW * 512 + (i * Cfg::kChunks + c) * 512);
+            }
+            const uint32_t st = smem_u32(tiles + s * Cfg::kStageBytes);
+            const uint64_t dw = smem_desc_sw128(st), da = smem_desc_sw128(st + Cfg::kTileBytes);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              // slice j's scales: all four bytes of word j (nvfp4), half j % 2 of word j / 2 (mxfp4), byte j (mxfp8)
+              const int word = kFmt == kFmtNvfp4 ? j : (kFmt == kFmtMxfp4 ? j / 2 : 0);
+              const uint32_t id = kFmt == kFmtNvfp4 ? 0u : (kFmt == kFmtMxfp4 ? 2u * (j % 2) : j);
+              mx_mma<kFmt, kPair>(d, dw + 2 * j, da + 2 * j, mx_idesc<kFmt, kPair>(nmma, id), t_w + 4 * word,
+                                  t_a + word * Cfg::kChunks * 4, (k > k0 || j > 0) ? 1u : 0u);
+            }
+            mx_commit<kPair>(&ctl->empty[s]);
+            if (group_ends) mx_commit<kPair>(&ctl->sf_empty[gs]);
           }
-          const uint32_t st = smem_u32(tiles + s * Cfg::kStageBytes);
-          const uint64_t dw = smem_desc_sw128(st), da = smem_desc_sw128(st + Cfg::kTileBytes);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // slice j's scales: all four bytes of word j (nvfp4), half j % 2 of word j / 2 (mxfp4), byte j (mxfp8)
-            const int word = kFmt == kFmtNvfp4 ? j : (kFmt == kFmtMxfp4 ? j / 2 : 0);
-            const uint32_t id = kFmt == kFmtNvfp4 ? 0u : (kFmt == kFmtMxfp4 ? 2u * (j % 2) : j);
-            mx_mma<kFmt>(d, dw + 2 * j, da + 2 * j, mx_idesc<kFmt>(nmma, id), t_w + 4 * word,
-                         t_a + word * Cfg::kChunks * 4, (k > k0 || j > 0) ? 1u : 0u);
-          }
-          mma_commit(&ctl->empty[s]);
+          __syncwarp();
+          if (group_ends) ++grp;
         }
         if (mx_aborted(ctl)) break;
-        mma_commit(&ctl->tfull[tile & 1u]);
+        if (el) mx_commit<kPair>(&ctl->tfull[tile & 1u]);
+        __syncwarp();
       }
       if (mx_aborted(ctl) && it > 0) {
-        mma_commit(&ctl->mma_done);
+        if (el) mx_commit<kPair>(&ctl->mma_done);
         mbar_wait_bounded(&ctl->mma_done, 0, kMxWaitNs);
       }
     }
   } else if (warp < kMxSfWarp0 + kMxSfWarps) {
     // ======================= scale loaders =======================
-    const int me = warp - kMxSfWarp0;
+    // Four stages at a time into one of two slots: lane 8 j + r of warp b
+    // loads stage j's words of rows 8 b + r, + 32, + 64, + 96 of every
+    // 128-row group (four lanes read a row's neighbouring words) and stores
+    // each word's four rows as one 16-byte piece.
+    const int r0 = (warp - kMxSfWarp0) * 8 + (lane & 7), j = lane >> 3;
     const auto mode_of = [&](const uint8_t* b) {
       const uint64_t m = reinterpret_cast<uint64_t>(b) | static_cast<uint64_t>(p.nsc);
       return (m & (4 * kW - 1)) == 0 ? 2 : ((m & 3) == 0 ? 1 : 0);
     };
     const int mode_w = mode_of(p.sw), mode_a = mode_of(p.sa);
-    uint32_t it = 0;
+    uint32_t grp = 0;
     bool ok = true;
     for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step) {
-      const MxUnit x = mx_unit(ctl, p, u, ntn);
-      const uint8_t* bw = p.sw + (static_cast<int64_t>(x.e) * p.N + x.n0) * p.nsc;
+      const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+      const int n0 = x.n0 + my_n;
+      const uint8_t* bw = p.sw + (static_cast<int64_t>(x.e) * p.N + n0) * p.nsc;
       const uint8_t* ba = p.sa + static_cast<int64_t>(x.row0) * p.nsc;
-      for (int k = k0; k < k1; ++k, ++it) {
-        if (static_cast<int>(it % kMxSfWarps) != me) continue;
-        const int s = it % kS;
-        const int at = k * 4 * kW, left = p.nsc - at;
-        uint32_t w[4][kW], a[Cfg::kChunks][4][kW];
-        // global loads first: they need no free stage
-        mx_sf_load<kW>(bw + at, p.nsc, p.N - x.n0, left, mode_w, lane, w);
+      for (int k = k0; k < k1; k += 4, ++grp) {
+        const int at = (k + j) * 4 * kW, left = k + j < k1 ? p.nsc - at : 0;
+        uint32_t w[1 + Cfg::kChunks][4][kW];
 #pragma unroll
-        for (int c = 0; c < Cfg::kChunks; ++c)
-          mx_sf_load<kW>(ba + at + static_cast<int64_t>(c) * 128 * p.nsc, p.nsc, x.cnt - c * 128, left, mode_a, lane, a[c]);
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs));
+        for (int q = 0; q < 4; ++q) {
+          const int r = r0 + 32 * q;
+          mx_sf_load<kW>(bw + static_cast<int64_t>(r) * p.nsc + at, r < p.N - n0 ? left : 0, mode_w, w[0][q]);
+#pragma unroll
+          for (int c = 0; c < Cfg::kChunks; ++c)
+            mx_sf_load<kW>(ba + static_cast<int64_t>(c * 128 + r) * p.nsc + at, c * 128 + r < x.cnt ? left : 0, mode_a,
+                           w[1 + c][q]);
+        }
+        const uint32_t gs = grp & 1u;
+        ok = all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp >> 1) & 1u) ^ 1u, kMxWaitNs));
         if (!ok) { mx_abort(ctl); break; }
-        uint8_t* sf = sfs + s * Cfg::kSfBytes;
-        mx_sf_store<kW>(sf, 512, lane, w);
+        uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
 #pragma unroll
-        for (int c = 0; c < Cfg::kChunks; ++c) mx_sf_store<kW>(sf + kW * 512 + c * 512, Cfg::kChunks * 512, lane, a[c]);
+        for (int i = 0; i < kW; ++i) {
+          *reinterpret_cast<uint4*>(sf + i * 512) = make_uint4(w[0][0][i], w[0][1][i], w[0][2][i], w[0][3][i]);
+#pragma unroll
+          for (int c = 0; c < Cfg::kChunks; ++c)
+            *reinterpret_cast<uint4*>(sf + kW * 512 + (i * Cfg::kChunks + c) * 512) =
+                make_uint4(w[1 + c][0][i], w[1 + c][1][i], w[1 + c][2][i], w[1 + c][3][i]);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->full[s]);
+        if (lane == 0) mx_arrive<kPair>(&ctl->sf_full[gs]);
       }
     }
   } else {
@@ -453,13 +561,13 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     const int ovc = shared_cols > 0 ? (shared_cols + 15) / 16 : 0;
     uint32_t tile = 0;
     for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step, ++tile) {
-      const MxUnit x = mx_unit(ctl, p, u, ntn);
+      const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
       const uint32_t buf = tile & 1u;
       const float alpha = p.alpha ? __ldg(p.alpha + x.e) : 1.0f;
       if (p.split > 1 && tile > 0) {  // the cluster has read this CTA's last partial sums
-        if (!__all_sync(0xffffffffu, cluster_wait_bounded(&ctl->part_free, (tile - 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+        if (!all_lanes(cluster_wait_bounded(&ctl->part_free, (tile - 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
       }
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctl->tfull[buf], (tile >> 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+      if (!all_lanes(mbar_wait_bounded(&ctl->tfull[buf], (tile >> 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
       __syncwarp();
       tc_fence_after();
       bool freed = false;
@@ -468,7 +576,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         if (!freed && i >= ovc) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->acc_free);
+          if (lane == 0) mx_arrive<kPair>(&ctl->acc_free);
           freed = true;
         }
         const int c = (buf == 0 ? nch - 1 - i : i) * 16;
@@ -478,21 +586,21 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         if (p.split > 1) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(c + j) * kMxTileN + nl] = v[j];
-        } else if (x.n0 + nl < p.N) {
+        } else if (x.n0 + my_n + nl < p.N) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c + j < x.cnt) mx_out_store(p, static_cast<int64_t>(x.row0) + c + j, x.n0 + nl, v[j] * alpha);
+            if (c + j < x.cnt) mx_out_store(p, static_cast<int64_t>(x.row0) + c + j, x.n0 + my_n + nl, v[j] * alpha);
         }
       }
       if (!freed) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->acc_free);
+        if (lane == 0) mx_arrive<kPair>(&ctl->acc_free);
       }
       if (p.split > 1) {
         epi_bar_sync();
         if (etid < p.split) cluster_arrive_remote(cluster_map(smem_u32(&ctl->part_ready), etid));
-        if (!__all_sync(0xffffffffu, cluster_wait_bounded(&ctl->part_ready, tile & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+        if (!all_lanes(cluster_wait_bounded(&ctl->part_ready, tile & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
         // tokens rank, rank + split, ...: a warp a token, four weight rows a lane
         const int n = x.n0 + lane * 4;
         for (int t = rank + (warp - kMxEpiWarp0) * p.split; t < x.cnt; t += kMxEpiWarps * p.split) {
@@ -516,20 +624,20 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 
   tc_fence_before();
   __syncwarp();
-  if (p.split > 1)
-    cluster_sync_all();  // no CTA leaves while another may read its sums
+  if (clustered)
+    cluster_sync_all();  // no CTA leaves while another may use its shared memory or TMEM
   else
     __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    mx_tmem_dealloc<kPair>(tmem);
   }
 }
 
-template <int kFmt, int kNT>
+template <int kFmt, int kNT, bool kPair>
 cudaError_t mx_gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const MxGemmArgs& p, int grid, cudaStream_t s) {
-  using Cfg = MxCfg<kFmt, kNT>;
+  using Cfg = MxCfg<kFmt, kNT, kPair>;
   static_assert(Cfg::kSmem + sizeof(MxCtl) <= 232448, "shared memory of a CTA");
   // the shared-memory opt-in is an attribute of the function on a device: one bit per device that has it
   static std::atomic<uint64_t> configured{0};
@@ -538,7 +646,7 @@ cudaError_t mx_gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const M
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!(configured.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(mx_gemm_kernel<kFmt, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(mx_gemm_kernel<kFmt, kNT, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(Cfg::kSmem));
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_relaxed);
@@ -552,22 +660,22 @@ cudaError_t mx_gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const M
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.x = kPair ? 2 : p.split;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<kFmt, kNT>, mw, ma, p);
+  cfg.numAttrs = kPair || p.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<kFmt, kNT, kPair>, mw, ma, p);
 }
 
 template <int kFmt>
-cudaError_t mx_gemm_launch_nt(int nt, const CUtensorMap& mw, const CUtensorMap& ma, const MxGemmArgs& p, int grid,
+cudaError_t mx_gemm_launch_nt(const MxPlan& pl, const CUtensorMap& mw, const CUtensorMap& ma, const MxGemmArgs& p,
                               cudaStream_t s) {
-  switch (nt) {
-    case 32: return mx_gemm_launch<kFmt, 32>(mw, ma, p, grid, s);
-    case 64: return mx_gemm_launch<kFmt, 64>(mw, ma, p, grid, s);
-    case 128: return mx_gemm_launch<kFmt, 128>(mw, ma, p, grid, s);
-    default: return mx_gemm_launch<kFmt, 256>(mw, ma, p, grid, s);
+  if (pl.pair) return mx_gemm_launch<kFmt, 256, true>(mw, ma, p, pl.grid, s);
+  switch (pl.nt) {
+    case 32: return mx_gemm_launch<kFmt, 32, false>(mw, ma, p, pl.grid, s);
+    case 64: return mx_gemm_launch<kFmt, 64, false>(mw, ma, p, pl.grid, s);
+    default: return mx_gemm_launch<kFmt, 128, false>(mw, ma, p, pl.grid, s);
   }
 }
 
@@ -577,6 +685,9 @@ cudaError_t mx_gemm_launch_nt(int nt, const CUtensorMap& mw, const CUtensorMap& 
 // One run of rows: the tile width that gives the least (waves of CTAs) x
 // (rows loaded per stage). Several runs, whose lengths only the device knows:
 // by their mean length.
+#ifndef MX_PAIR_ABOVE
+#define MX_PAIR_ABOVE 128
+#endif
 MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs) {
   const int sms = device_sm_count();
   const int64_t ntn = (N + kMxTileN - 1) / kMxTileN;
@@ -597,6 +708,17 @@ MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs) {
       }
     }
   }
+  // wide tiles: a pair of CTAs, each with half of the tokens in shared memory
+  pl.pair = pl.tn > MX_PAIR_ABOVE;
+  if (pl.pair) {
+    const int64_t tiles = (N + 2 * kMxTileN - 1) / (2 * kMxTileN) * (rows / pl.tn + (runs ? (experts < rows ? experts : rows) : 1));
+    pl.nt = 256;
+    pl.split = 1;
+    pl.grid = static_cast<int>(2 * (tiles < sms / 2 ? tiles : sms / 2));
+    pl.box_rows = pl.tn / 2;
+    return pl;
+  }
+  pl.box_rows = pl.tn;
   pl.nt = pl.tn <= 32 ? 32 : pl.tn <= 64 ? 64 : pl.tn <= 128 ? 128 : 256;
   const int64_t busy = runs ? (experts < rows ? experts : rows) : 1;             // runs that can have rows
   const int64_t most = (rows / pl.tn + busy) * ntn;                              // no call has more tiles
@@ -627,9 +749,9 @@ cudaError_t launch_mx_gemm(const CUtensorMap& map_w, const CUtensorMap& map_a, c
   p.tn = pl.tn;
   p.split = pl.split;
   switch (c.fmt) {
-    case kFmtNvfp4: return mx_gemm_launch_nt<kFmtNvfp4>(pl.nt, map_w, map_a, p, pl.grid, s);
-    case kFmtMxfp4: return mx_gemm_launch_nt<kFmtMxfp4>(pl.nt, map_w, map_a, p, pl.grid, s);
-    default: return mx_gemm_launch_nt<kFmtMxfp8>(pl.nt, map_w, map_a, p, pl.grid, s);
+    case kFmtNvfp4: return mx_gemm_launch_nt<kFmtNvfp4>(pl, map_w, map_a, p, s);
+    case kFmtMxfp4: return mx_gemm_launch_nt<kFmtMxfp4>(pl, map_w, map_a, p, s);
+    default: return mx_gemm_launch_nt<kFmtMxfp8>(pl, map_w, map_a, p, s);
   }
 }
 
