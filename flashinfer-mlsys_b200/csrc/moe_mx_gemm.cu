@@ -27,6 +27,7 @@
 // share of the tokens over the cluster's shared memory in rank order, so there
 // is no scratch, no atomics, and one answer.
 #include <atomic>
+#include <type_traits>
 
 #include "moe_kernels.h"
 #include "moe_mx.cuh"
@@ -52,14 +53,15 @@ struct MxCfg {
   static constexpr int kTileBytes = kMxTileN * kMxStageK;
   static constexpr int kStageBytes = kTileBytes + (kPair ? kNT / 2 : kNT) * kMxStageK;  // a pair halves the tokens
   static constexpr int kSfBytes = kW * 512 * (1 + kChunks);
-  static constexpr int kStages = kPair ? 5 : (kNT > 64 ? 5 : (kNT > 32 ? 6 : 8));
+  static constexpr int kStages = kPair ? 4 : (kNT > 64 ? 5 : (kNT > 32 ? 6 : 8));
   static constexpr int kGroupBytes = 4 * kSfBytes;  // scales of four stages
+  static constexpr int kGroups = kPair ? (kW > 2 ? 3 : 4) : 2;  // slots of them
   static constexpr int kSfCols = kW * 4 * (1 + kChunks);  // TMEM columns of one slot
   static constexpr int kAccCols = (512 - 2 * kSfCols) & ~31;
   static constexpr bool kOwnPart = kNT <= 64;             // room for the split's partial sums beside the ring
   static constexpr int kPartBytes = kNT * kMxTileN * 4;
   static constexpr size_t kSmem =
-      1024 + (size_t)kStages * kStageBytes + 2 * kGroupBytes + (kOwnPart ? kPartBytes : 0);
+      1024 + (size_t)kStages * kStageBytes + kGroups * kGroupBytes + (kOwnPart ? kPartBytes : 0);
   static_assert(kOwnPart || kPartBytes <= kStages * kStageBytes, "partial sums reuse the ring");
 };
 
@@ -79,7 +81,7 @@ struct MxGemmArgs {
 };
 
 struct __align__(16) MxCtl {
-  uint64_t full[8], empty[8], sf_full[2], sf_empty[2], tfull[2], acc_free, part_ready, part_free, mma_done;
+  uint64_t full[8], empty[8], sf_full[4], sf_empty[4], peer_sf[4], tfull[2], acc_free, peer_acc, part_ready, part_free, mma_done;
   uint32_t tmem_base;
   int abort_flag;
   int start[kMxMaxExperts + 1];   // first row of each run
@@ -246,20 +248,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "memory");
   return v;
 }
-// A barrier of the first CTA of a pair, on which both arrive; otherwise this CTA's own.
+// This CTA's barrier and, in a pair, the one that the second CTA's relay arrives on.
 template <bool kPair>
-__device__ __forceinline__ void mx_arrive(uint64_t* bar) {
-  if constexpr (kPair)
-    cluster_arrive_remote(cluster_map(smem_u32(bar), 0));
-  else
-    mbar_arrive(bar);
-}
-template <bool kPair>
-__device__ __forceinline__ bool mx_wait(uint64_t* bar, uint32_t parity) {
-  if constexpr (kPair)
-    return cluster_wait_bounded(bar, parity, kMxWaitNs);
-  else
-    return mbar_wait_bounded(bar, parity, kMxWaitNs);
+__device__ __forceinline__ bool mx_wait_both(uint64_t* own, uint64_t* peer, uint32_t parity) {
+  if (!mbar_wait_bounded(own, parity, kMxWaitNs)) return false;
+  if constexpr (kPair) return cluster_wait_bounded(peer, parity, kMxWaitNs);
+  return true;
 }
 
 __device__ __forceinline__ void epi_bar_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -276,24 +270,27 @@ __device__ __forceinline__ void mx_out_store(const MxGemmArgs& p, int64_t row, i
 }
 
 // The scale words of one row and stage: `left` scales remain in the row from
-// `s` on (none: zeros). mode 2: rows are whole stages, one vector load; 1:
-// words; 0: bytes (any row length).
-template <int kW>
-__device__ __forceinline__ void mx_sf_load(const uint8_t* s, int left, int mode, uint32_t (&w)[kW]) {
+// `s` on (none: zeros). kVec: rows are whole stages, aligned to one; otherwise
+// words where every row is, or bytes.
+template <int kW, bool kVec>
+__device__ __forceinline__ void mx_sf_load(const uint8_t* s, int left, bool words, uint32_t (&w)[kW]) {
 #pragma unroll
   for (int i = 0; i < kW; ++i) w[i] = 0;
-  if (left <= 0) return;
-  if (mode == 2) {
-    if constexpr (kW == 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (kW == 2) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-      w[0] = v.x, w[1] = v.y;
-    } else {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+  if constexpr (kVec) {
+    if (left > 0) {
+      if constexpr (kW == 4) {
+        uint4 v;  // volatile: stays before the wait for the slot
+        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(s));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else if constexpr (kW == 2) {
+        uint2 v;
+        asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(s));
+        w[0] = v.x, w[1] = v.y;
+      } else {
+        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[0]) : "l"(s));
+      }
     }
-  } else if (mode == 1) {
+  } else if (words) {
 #pragma unroll
     for (int i = 0; i < kW; ++i)
       if (4 * i < left) w[i] = __ldg(reinterpret_cast<const uint32_t*>(s) + i);
@@ -324,7 +321,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   MxCtl* ctl = &ctl_;
   uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sfs = tiles + kS * Cfg::kStageBytes;
-  float* part = reinterpret_cast<float*>(Cfg::kOwnPart ? sfs + 2 * Cfg::kGroupBytes : tiles);
+  float* part = reinterpret_cast<float*>(Cfg::kOwnPart ? sfs + Cfg::kGroups * Cfg::kGroupBytes : tiles);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // a unit is one tile of weight rows x tokens, and belongs to a cluster: a
@@ -344,13 +341,15 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&ctl->sf_full[b], kPair ? 2 * kMxSfWarps : kMxSfWarps);
+    for (int b = 0; b < Cfg::kGroups; ++b) {
+      mbar_init(&ctl->sf_full[b], kMxSfWarps);
+      mbar_init(&ctl->peer_sf[b], 1);
       mbar_init(&ctl->sf_empty[b], 1);
     }
     mbar_init(&ctl->tfull[0], 1);
     mbar_init(&ctl->tfull[1], 1);
-    mbar_init(&ctl->acc_free, kPair ? 2 * kMxEpiWarps : kMxEpiWarps);
+    mbar_init(&ctl->acc_free, kMxEpiWarps);
+    mbar_init(&ctl->peer_acc, 1);
     mbar_init(&ctl->part_ready, p.split);
     mbar_init(&ctl->part_free, p.split);
     mbar_init(&ctl->mma_done, 1);
@@ -456,14 +455,20 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         const int nmma = (x.cnt + 15) & ~15;
         const uint32_t d = acc_at[tile & 1u];
         // the tile before last has left this accumulator and the last one the columns they share
-        if (tile > 0 && !all_lanes(mx_wait<kPair>(&ctl->acc_free, (tile - 1) & 1u))) { mx_abort(ctl); break; }
+        if (tile > 0 && !all_lanes(mx_wait_both<kPair>(&ctl->acc_free, &ctl->peer_acc, (tile - 1) & 1u))) {
+          mx_abort(ctl);
+          break;
+        }
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % kS, kg = (k - k0) & 3;
-          const uint32_t gs = grp & 1u;
-          if (kg == 0 && !all_lanes(mx_wait<kPair>(&ctl->sf_full[gs], (grp >> 1) & 1u))) { mx_abort(ctl); break; }
+          const uint32_t gs = grp % Cfg::kGroups;
+          if (kg == 0 && !all_lanes(mx_wait_both<kPair>(&ctl->sf_full[gs], &ctl->peer_sf[gs], (grp / Cfg::kGroups) & 1u))) {
+            mx_abort(ctl);
+            break;
+          }
           // the TMEM scale slot's last readers have finished (two stages back)
           if (it >= 2 && !all_lanes(mbar_wait_bounded(&ctl->empty[(it - 2) % kS], ((it - 2) / kS) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
-          if (!all_lanes(mx_wait<kPair>(&ctl->full[s], (it / kS) & 1u))) { mx_abort(ctl); break; }
+          if (!all_lanes(mbar_wait_bounded(&ctl->full[s], (it / kS) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
           tc_fence_after();
           const bool group_ends = kg == 3 || k == k1 - 1;
           if (el) {
@@ -501,6 +506,27 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         if (el) mx_commit<kPair>(&ctl->mma_done);
         mbar_wait_bounded(&ctl->mma_done, 0, kMxWaitNs);
       }
+    } else {
+      // The second CTA's relay: its scale loaders and its epilogue arrive on
+      // barriers of their own CTA, and this warp passes that on to the first
+      // CTA. A release at cluster scope takes some 1400 cycles here; in the
+      // scale loaders it held up every group (120 -> 111 us at 8192 x 7168 x 4096 nvfp4).
+      uint32_t tile = 0, grp = 0;
+      bool ok = true;
+      for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step, ++tile) {
+        if (tile > 0) {
+          ok = all_lanes(mbar_wait_bounded(&ctl->acc_free, (tile - 1) & 1u, kMxWaitNs));
+          if (!ok) break;
+          if (lane == 0) cluster_arrive_remote(cluster_map(smem_u32(&ctl->peer_acc), 0));
+        }
+        for (int k = k0; k < k1; k += 4, ++grp) {
+          const uint32_t gs = grp % Cfg::kGroups;
+          ok = all_lanes(mbar_wait_bounded(&ctl->sf_full[gs], (grp / Cfg::kGroups) & 1u, kMxWaitNs));
+          if (!ok) break;
+          if (lane == 0) cluster_arrive_remote(cluster_map(smem_u32(&ctl->peer_sf[gs]), 0));
+        }
+      }
+      if (!ok) mx_abort(ctl);
     }
   } else if (warp < kMxSfWarp0 + kMxSfWarps) {
     // ======================= scale loaders =======================
@@ -509,33 +535,39 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     // 128-row group (four lanes read a row's neighbouring words) and stores
     // each word's four rows as one 16-byte piece.
     const int r0 = (warp - kMxSfWarp0) * 8 + (lane & 7), j = lane >> 3;
-    const auto mode_of = [&](const uint8_t* b) {
-      const uint64_t m = reinterpret_cast<uint64_t>(b) | static_cast<uint64_t>(p.nsc);
-      return (m & (4 * kW - 1)) == 0 ? 2 : ((m & 3) == 0 ? 1 : 0);
-    };
-    const int mode_w = mode_of(p.sw), mode_a = mode_of(p.sa);
-    uint32_t grp = 0;
-    bool ok = true;
-    for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step) {
-      const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+    const uint64_t low =
+        reinterpret_cast<uint64_t>(p.sw) | reinterpret_cast<uint64_t>(p.sa) | static_cast<uint64_t>(p.nsc);
+    const bool words = (low & 3) == 0;
+    // one loop for each kind of row, so that the usual one has no branches
+    // among its loads: with them it waited for every load where it stood
+    const auto loop = [&](auto vec) {
+    constexpr bool kVec = decltype(vec)::value;
+    // the words of stages k .. k + 3 of unit x
+    const auto load = [&](const MxUnit& x, int k, uint32_t (&w)[1 + Cfg::kChunks][4][kW]) {
       const int n0 = x.n0 + my_n;
       const uint8_t* bw = p.sw + (static_cast<int64_t>(x.e) * p.N + n0) * p.nsc;
       const uint8_t* ba = p.sa + static_cast<int64_t>(x.row0) * p.nsc;
+      const int at = (k + j) * 4 * kW, left = k + j < k1 ? p.nsc - at : 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = r0 + 32 * q;
+        mx_sf_load<kW, kVec>(bw + static_cast<int64_t>(r) * p.nsc + at, r < p.N - n0 ? left : 0, words, w[0][q]);
+#pragma unroll
+        for (int c = 0; c < Cfg::kChunks; ++c)
+          mx_sf_load<kW, kVec>(ba + static_cast<int64_t>(c * 128 + r) * p.nsc + at, c * 128 + r < x.cnt ? left : 0, words,
+                               w[1 + c][q]);
+      }
+    };
+    uint32_t w[1 + Cfg::kChunks][4][kW];
+    uint32_t grp = 0;
+    for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
+      const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+      bool ok = true;
       for (int k = k0; k < k1; k += 4, ++grp) {
-        const int at = (k + j) * 4 * kW, left = k + j < k1 ? p.nsc - at : 0;
-        uint32_t w[1 + Cfg::kChunks][4][kW];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = r0 + 32 * q;
-          mx_sf_load<kW>(bw + static_cast<int64_t>(r) * p.nsc + at, r < p.N - n0 ? left : 0, mode_w, w[0][q]);
-#pragma unroll
-          for (int c = 0; c < Cfg::kChunks; ++c)
-            mx_sf_load<kW>(ba + static_cast<int64_t>(c * 128 + r) * p.nsc + at, c * 128 + r < x.cnt ? left : 0, mode_a,
-                           w[1 + c][q]);
-        }
-        const uint32_t gs = grp & 1u;
-        ok = all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp >> 1) & 1u) ^ 1u, kMxWaitNs));
-        if (!ok) { mx_abort(ctl); break; }
+        load(x, k, w);  // under way while the slot is still being read
+        const uint32_t gs = grp % Cfg::kGroups;
+        ok = all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp / Cfg::kGroups) & 1u) ^ 1u, kMxWaitNs));
+        if (!ok) break;
         uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
 #pragma unroll
         for (int i = 0; i < kW; ++i) {
@@ -547,9 +579,15 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mx_arrive<kPair>(&ctl->sf_full[gs]);
+        if (lane == 0) mbar_arrive(&ctl->sf_full[gs]);
       }
+      if (!ok) { mx_abort(ctl); break; }
     }
+    };
+    if ((low & (4 * kW - 1)) == 0)
+      loop(std::true_type{});
+    else
+      loop(std::false_type{});
   } else {
     // ======================= epilogue (8 warps) =======================
     const int q = warp & 3, half = (warp - kMxEpiWarp0) >> 2;
@@ -576,7 +614,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         if (!freed && i >= ovc) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mx_arrive<kPair>(&ctl->acc_free);
+          if (lane == 0) mbar_arrive(&ctl->acc_free);
           freed = true;
         }
         const int c = (buf == 0 ? nch - 1 - i : i) * 16;
@@ -595,7 +633,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (!freed) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mx_arrive<kPair>(&ctl->acc_free);
+        if (lane == 0) mbar_arrive(&ctl->acc_free);
       }
       if (p.split > 1) {
         epi_bar_sync();
