@@ -58,6 +58,9 @@ struct MxCfg {
   static constexpr int kGroups = kPair ? (kW > 2 ? 3 : 4) : 2;  // slots of them
   static constexpr int kSfCols = kW * 4 * (1 + kChunks);  // TMEM columns of one slot
   static constexpr int kAccCols = (512 - 2 * kSfCols) & ~31;
+  // 16-column pieces of the overlap of two widest accumulators that a warp of the epilogue holds
+  static constexpr int kShared = kNT - ((kAccCols - kNT) & ~31);
+  static constexpr int kHeld = kShared > 0 ? (kShared / 16 + 1) / 2 : 0;
   static constexpr bool kOwnPart = kNT <= 64;             // room for the split's partial sums beside the ring
   static constexpr int kPartBytes = kNT * kMxTileN * 4;
   static constexpr size_t kSmem =
@@ -223,6 +226,9 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_arrive_remote(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive_remote_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
 __device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   const uint64_t t0 = global_timer_ns();
   while (true) {
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     mbar_init(&ctl->tfull[0], 1);
     mbar_init(&ctl->tfull[1], 1);
     mbar_init(&ctl->acc_free, kMxEpiWarps);
-    mbar_init(&ctl->peer_acc, 1);
+    mbar_init(&ctl->peer_acc, kMxEpiWarps);
     mbar_init(&ctl->part_ready, p.split);
     mbar_init(&ctl->part_free, p.split);
     mbar_init(&ctl->mma_done, 1);
@@ -507,18 +513,13 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         mbar_wait_bounded(&ctl->mma_done, 0, kMxWaitNs);
       }
     } else {
-      // The second CTA's relay: its scale loaders and its epilogue arrive on
-      // barriers of their own CTA, and this warp passes that on to the first
-      // CTA. A release at cluster scope takes some 1400 cycles here; in the
-      // scale loaders it held up every group (120 -> 111 us at 8192 x 7168 x 4096 nvfp4).
-      uint32_t tile = 0, grp = 0;
+      // The second CTA's relay: its scale loaders arrive on barriers of their
+      // own CTA, and this warp passes that on to the first CTA. A release at
+      // cluster scope takes some 1400 cycles here; in the scale loaders it
+      // held up every group (120 -> 111 us at 8192 x 7168 x 4096 nvfp4).
+      uint32_t grp = 0;
       bool ok = true;
-      for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step, ++tile) {
-        if (tile > 0) {
-          ok = all_lanes(mbar_wait_bounded(&ctl->acc_free, (tile - 1) & 1u, kMxWaitNs));
-          if (!ok) break;
-          if (lane == 0) cluster_arrive_remote(cluster_map(smem_u32(&ctl->peer_acc), 0));
-        }
+      for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step) {
         for (int k = k0; k < k1; k += 4, ++grp) {
           const uint32_t gs = grp % Cfg::kGroups;
           ok = all_lanes(mbar_wait_bounded(&ctl->sf_full[gs], (grp / Cfg::kGroups) & 1u, kMxWaitNs));
@@ -608,19 +609,10 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (!all_lanes(mbar_wait_bounded(&ctl->tfull[buf], (tile >> 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
       __syncwarp();
       tc_fence_after();
-      bool freed = false;
-      // buffer 0 shares its last columns with buffer 1's first
-      for (int i = half; i < nch; i += 2) {
-        if (!freed && i >= ovc) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->acc_free);
-          freed = true;
-        }
-        const int c = (buf == 0 ? nch - 1 - i : i) * 16;
-        if (c >= x.cnt) continue;
-        float v[16];
-        tmem_ld_32x32b_x16(acc_at[buf] + t_lane + c, v);
+      // buffer 0 shares its last columns with buffer 1's first: those go to
+      // registers and are given back before anything is stored
+      const auto column = [&](int i) { return (buf == 0 ? nch - 1 - i : i) * 16; };
+      const auto store = [&](int c, const float (&v)[16]) {
         if (p.split > 1) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(c + j) * kMxTileN + nl] = v[j];
@@ -629,11 +621,32 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
           for (int j = 0; j < 16; ++j)
             if (c + j < x.cnt) mx_out_store(p, static_cast<int64_t>(x.row0) + c + j, x.n0 + my_n + nl, v[j] * alpha);
         }
+      };
+      float head[Cfg::kHeld > 0 ? Cfg::kHeld : 1][16];
+#pragma unroll
+      for (int h = 0; h < Cfg::kHeld; ++h) {
+        const int i = half + 2 * h;
+        if (i < ovc && column(i) < x.cnt) tmem_ld_32x32b_x16(acc_at[buf] + t_lane + column(i), head[h]);
       }
-      if (!freed) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->acc_free);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (!kPair || rank == 0)
+          mbar_arrive(&ctl->acc_free);
+        else  // nothing in memory to publish: the loads from TMEM are complete
+          cluster_arrive_remote_relaxed(cluster_map(smem_u32(&ctl->peer_acc), 0));
+      }
+#pragma unroll
+      for (int h = 0; h < Cfg::kHeld; ++h) {
+        const int i = half + 2 * h;
+        if (i < ovc && column(i) < x.cnt) store(column(i), head[h]);
+      }
+      for (int i = half + (ovc > half ? (ovc - half + 1) / 2 * 2 : 0); i < nch; i += 2) {
+        const int c = column(i);
+        if (c >= x.cnt) continue;
+        float v[16];
+        tmem_ld_32x32b_x16(acc_at[buf] + t_lane + c, v);
+        store(c, v);
       }
       if (p.split > 1) {
         epi_bar_sync();
