@@ -18,7 +18,7 @@ bool valid_dt(int dt) { return dt == MOE_DT_BF16 || dt == MOE_DT_FP16 || dt == M
 int64_t dt_size(int dt) { return dt == MOE_DT_FP32 ? 4 : 2; }
 
 int rows_cols(int64_t rows, int64_t cols, int fmt, int dt) {
-  if (rows < 0 || rows > kMaxRows || cols <= 0 || cols > kMaxCols || cols % kMxUnit || !valid_fmt(fmt) || !valid_dt(dt))
+  if (rows < 0 || rows > kMaxRows || cols <= 0 || cols > kMaxCols || cols % kMxCols || !valid_fmt(fmt) || !valid_dt(dt))
     return MOE_ERR_INVALID_ARG;
   return MOE_OK;
 }
@@ -30,11 +30,9 @@ int strided(const void* p, int64_t ld, int64_t rows, int64_t cols, int dt) {
   return MOE_OK;
 }
 
-int packed(const void* q, const void* scale, int fmt) {
+int packed(const void* q, const void* scale) {
   if (!q || !scale) return MOE_ERR_INVALID_ARG;
-  // quantisers write an nvfp4 unit's two scales as one 16-bit word
-  if (!aligned(q, 16) || (fmt == MOE_MX_NVFP4 && !aligned(scale, 2))) return MOE_ERR_ALIGNMENT;
-  return MOE_OK;
+  return aligned(q, 16) ? MOE_OK : MOE_ERR_ALIGNMENT;
 }
 
 int tensor_scale(const float* g, int fmt) {
@@ -111,7 +109,7 @@ int moe_fp8_ds_quantize_mx(const void* x, int dtype, int64_t rows, int64_t cols,
   MOE_TRY(tensor_scale(global_scale, fmt));
   if (rows == 0) return check_device_sm100();
   MOE_TRY(strided(x, x_ld, rows, cols, dtype));
-  MOE_TRY(packed(q_out, scale_out, fmt));
+  MOE_TRY(packed(q_out, scale_out));
   MOE_TRY(check_device_sm100());
   return cuda_rc(launch_mx_quant(x, dtype, x_ld, rows, cols, fmt, global_scale, q_out, scale_out,
                                  static_cast<cudaStream_t>(stream)));
@@ -123,7 +121,7 @@ int moe_fp8_ds_dequantize_mx(const void* q, const void* scale, int64_t rows, int
   MOE_TRY(tensor_scale(global_scale, fmt));
   if (rows == 0) return check_device_sm100();
   MOE_TRY(strided(x_out, x_ld, rows, cols, dtype));
-  MOE_TRY(packed(q, scale, fmt));
+  MOE_TRY(packed(q, scale));
   MOE_TRY(check_device_sm100());
   return cuda_rc(launch_mx_dequant(q, scale, rows, cols, fmt, global_scale, dtype, x_out, x_ld,
                                    static_cast<cudaStream_t>(stream)));
@@ -139,7 +137,7 @@ int moe_fp8_ds_add_norm_quantize_mx(const void* x, int64_t x_ld, void* residual,
   MOE_TRY(strided(x, x_ld, rows, cols, dtype));
   if (residual) MOE_TRY(strided(residual, residual_ld, rows, cols, dtype));
   if (!aligned(norm_weight, 16)) return MOE_ERR_ALIGNMENT;
-  MOE_TRY(packed(q_out, scale_out, fmt));
+  MOE_TRY(packed(q_out, scale_out));
   MOE_TRY(check_device_sm100());
   const MxNormCall c{x, x_ld, residual, residual_ld, norm_weight, eps, rows, cols, global_scale, q_out, scale_out};
   return cuda_rc(launch_mx_norm(c, fmt, dtype, static_cast<cudaStream_t>(stream)));

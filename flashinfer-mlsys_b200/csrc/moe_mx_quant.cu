@@ -1,10 +1,7 @@
 // moe_mx_quant.cu — rows of bf16, fp16 or fp32 to a microscaled format
 // (moe_mx.cuh) and back, and the residual add + RMSNorm that ends in one.
 //
-// All three are one pass over the data and HBM-bound. One thread owns one unit
-// (32 columns): a block's scale needs no exchange between threads, the packed
-// values leave as one or two 16-byte stores, and neighbouring threads' units
-// are adjacent, so every 32-byte sector is used whole.
+// All three are one pass over the data and HBM-bound.
 #include "moe_kernels.h"
 #include "moe_mx.cuh"
 
@@ -13,177 +10,270 @@ namespace moe {
 namespace {
 
 constexpr int kMxThreads = 256;
+constexpr int kQuantPer = 2;    // spans of a quantising thread, all loaded before the first is used
+constexpr int kDequantPer = 4;  // octets of a dequantising one
+constexpr int kMxOctet = 8;
 
-__device__ __forceinline__ void store_scale(void* scale, uint64_t unit, int per_unit, uint32_t sc) {
-  if (per_unit == 2)
-    static_cast<uint16_t*>(scale)[unit] = static_cast<uint16_t>(sc);
+// The span's packed words; the block's first lane stores its scale.
+template <int kFmt>
+__device__ __forceinline__ void mx_store_packed(uint8_t* q, uint8_t* scale, uint64_t span, const uint32_t* w,
+                                                uint32_t sc) {
+  if constexpr (kFmt == kFmtMxfp8)
+    reinterpret_cast<uint4*>(q)[span] = make_uint4(w[0], w[1], w[2], w[3]);
   else
-    static_cast<uint8_t*>(scale)[unit] = static_cast<uint8_t>(sc);
+    reinterpret_cast<uint2*>(q)[span] = make_uint2(w[0], w[1]);
+  constexpr int kLanes = mx_block(kFmt) / kMxSpan;
+  if (span % kLanes == 0) scale[span / kLanes] = static_cast<uint8_t>(sc);
 }
 
-// x [rows][x_ld] -> q, scale (both contiguous); `per_row` units a row.
+// Byte offset of piece `i` of kB bytes in rows `ld_bytes` apart (per_row pieces each).
+template <int kB>
+__device__ __forceinline__ int64_t mx_at(uint64_t i, uint32_t per_row, int64_t ld_bytes) {
+  if (ld_bytes == static_cast<int64_t>(per_row) * kB) return static_cast<int64_t>(i) * kB;
+  const uint64_t row = i / per_row;
+  return static_cast<int64_t>(row) * ld_bytes + static_cast<int64_t>(i - row * per_row) * kB;
+}
+
+// x [rows][x_ld] -> q, scale (both contiguous); `per_row` spans a row. Spans
+// past the end load nothing and take part in the shuffles only: a block never
+// straddles the end.
 template <int kFmt, int kDt>
 __global__ void __launch_bounds__(kMxThreads)
-    mx_quant_kernel(const uint8_t* __restrict__ x, int64_t x_ld_bytes, uint64_t units, uint32_t per_row,
-                    const float* __restrict__ global_scale, uint8_t* __restrict__ q, void* __restrict__ scale) {
-  const uint64_t u = blockIdx.x * static_cast<uint64_t>(kMxThreads) + threadIdx.x;
+    mx_quant_kernel(const uint8_t* __restrict__ x, int64_t x_ld_bytes, bool wide, uint64_t spans, uint32_t per_row,
+                    const float* __restrict__ global_scale, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  const uint64_t u0 = blockIdx.x * static_cast<uint64_t>(kMxThreads * kQuantPer) + threadIdx.x;
   griddep_wait();
   griddep_launch_dependents();
-  if (u >= units) return;
-  const uint64_t row = u / per_row;
-  const uint32_t c = static_cast<uint32_t>(u - row * per_row);
-  constexpr int kW = MxWords<kDt>::n;
-  uint32_t w[kW];
-  mx_load<kW>(x + row * x_ld_bytes + static_cast<uint64_t>(c) * (4 * kW), w);
-  const float g = (kFmt == kFmtNvfp4 && global_scale) ? __ldg(global_scale) : 1.0f;
-  float f[32];
-  mx_to_float<kDt>(w, f);
-  uint32_t am[2];
-  if constexpr (kDt == kDtFp32)
-    mx_amax<kFmt>(f, am);
-  else
-    mx_amax_packed<kFmt, kDt>(w, am);
-  uint32_t o[8];
-  const uint32_t sc = mx_quant_unit<kFmt>(f, am, g, o);
-  constexpr int kB = mx_unit_bytes(kFmt);
-  mx_store<kB / 4>(q + u * kB, o);
-  store_scale(scale, u, mx_unit_scales(kFmt), sc);
+  constexpr int kW = MxWords<kDt, kMxSpan>::n;
+  uint32_t w[kQuantPer][kW];
+#pragma unroll
+  for (int j = 0; j < kQuantPer; ++j) {
+    const uint64_t u = u0 + j * kMxThreads;
+    if (u < spans) {
+      mx_load<kW>(x + mx_at<4 * kW>(u, per_row, x_ld_bytes), wide, w[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kW; ++i) w[j][i] = 0;
+    }
+  }
+  const MxGlobal gl = mx_global(kFmt == kFmtNvfp4 ? global_scale : nullptr);
+#pragma unroll
+  for (int j = 0; j < kQuantPer; ++j) {
+    const uint64_t u = u0 + j * kMxThreads;
+    float f[kMxSpan];
+    mx_to_float<kDt>(w[j], f);
+    uint32_t am;
+    if constexpr (kDt == kDtFp32)
+      am = mx_span_max(f);
+    else
+      am = mx_span_max_packed<kDt>(w[j]);
+    am = mx_block_max<kFmt>(am);
+    uint32_t p[4];
+    const uint32_t sc = mx_quant_span<kFmt>(f, am, gl, p);
+    if (u < spans) mx_store_packed<kFmt>(q, scale, u, p, sc);
+  }
 }
 
 // q, scale (contiguous) -> x [rows][x_ld]: (value * scale) * global_scale in
 // float32 (the first product is exact), rounded once to the output's type.
 template <int kFmt, int kDt>
 __global__ void __launch_bounds__(kMxThreads)
-    mx_dequant_kernel(const uint8_t* __restrict__ q, const void* __restrict__ scale, uint64_t units, uint32_t per_row,
-                      const float* __restrict__ global_scale, uint8_t* __restrict__ x, int64_t x_ld_bytes) {
-  const uint64_t u = blockIdx.x * static_cast<uint64_t>(kMxThreads) + threadIdx.x;
+    mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, uint64_t octets,
+                      uint32_t per_row, const float* __restrict__ global_scale, uint8_t* __restrict__ x,
+                      int64_t x_ld_bytes, bool wide) {
+  const uint64_t o0 = blockIdx.x * static_cast<uint64_t>(kMxThreads * kDequantPer) + threadIdx.x;
   griddep_wait();
   griddep_launch_dependents();
-  if (u >= units) return;
-  const uint64_t row = u / per_row;
-  const uint32_t c = static_cast<uint32_t>(u - row * per_row);
-  constexpr int kB = mx_unit_bytes(kFmt);
-  uint32_t o[kB / 4];
-  mx_load<kB / 4>(q + u * kB, o);
-  float s[2];
-  if constexpr (kFmt == kFmtNvfp4) {
-    const float2 v = e4m3x2_to_f2(static_cast<const uint16_t*>(scale)[u]);
-    s[0] = v.x;
-    s[1] = v.y;
-  } else {
-    s[0] = s[1] = e8m0_to_f(static_cast<const uint8_t*>(scale)[u]);
-  }
-  const float g = (kFmt == kFmtNvfp4 && global_scale) ? __ldg(global_scale) : 1.0f;
-  float f[32];
+  constexpr int kLanes = mx_block(kFmt) / kMxOctet;
+  uint2 v[kDequantPer];
+  uint32_t sb[kDequantPer];
 #pragma unroll
-  for (int i = 0; i < kB / 4; ++i) {
-    if constexpr (kFmt == kFmtMxfp8) {
-      const float2 lo = e4m3x2_to_f2(o[i] & 0xFFFFu), hi = e4m3x2_to_f2(o[i] >> 16);
-      f[4 * i] = lo.x;
-      f[4 * i + 1] = lo.y;
-      f[4 * i + 2] = hi.x;
-      f[4 * i + 3] = hi.y;
-    } else {
-      e2m1x8_to_f8(o[i], f + 8 * i);
+  for (int j = 0; j < kDequantPer; ++j) {
+    const uint64_t o = o0 + j * kMxThreads;
+    v[j] = make_uint2(0, 0);
+    sb[j] = 0;
+    if (o < octets) {
+      if constexpr (kFmt == kFmtMxfp8)
+        v[j] = __ldcs(reinterpret_cast<const uint2*>(q) + o);
+      else
+        v[j].x = __ldcs(reinterpret_cast<const uint32_t*>(q) + o);
+      sb[j] = __ldg(scale + o / kLanes);
     }
   }
+  const float g = (kFmt == kFmtNvfp4 && global_scale) ? __ldg(global_scale) : 1.0f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    f[i] *= s[i / 16];
-    if (kFmt == kFmtNvfp4) f[i] *= g;
+  for (int j = 0; j < kDequantPer; ++j) {
+    const uint64_t o = o0 + j * kMxThreads;
+    if (o >= octets) continue;
+    float f[kMxOctet];
+    if constexpr (kFmt == kFmtMxfp8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t b = i ? v[j].y : v[j].x;
+        const float2 lo = e4m3x2_to_f2(b & 0xFFFFu), hi = e4m3x2_to_f2(b >> 16);
+        f[4 * i] = lo.x;
+        f[4 * i + 1] = lo.y;
+        f[4 * i + 2] = hi.x;
+        f[4 * i + 3] = hi.y;
+      }
+    } else {
+      e2m1x8_to_f8(v[j].x, f);
+    }
+    const float s = kFmt == kFmtNvfp4 ? e4m3x2_to_f2(sb[j]).x : e8m0_to_f(sb[j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] *= s;
+      if (kFmt == kFmtNvfp4) f[i] *= g;
+    }
+    constexpr int kW = MxWords<kDt, kMxOctet>::n;
+    uint32_t w[kW];
+    mx_from_float<kDt>(f, w);
+    mx_store<kW>(x + mx_at<4 * kW>(o, per_row, x_ld_bytes), wide, w);
   }
-  constexpr int kW = MxWords<kDt>::n;
-  uint32_t w[kW];
-  mx_from_float<kDt>(f, w);
-  mx_store<kW>(x + row * x_ld_bytes + static_cast<uint64_t>(c) * (4 * kW), w);
 }
 
-// h = T(residual + x) (written back), y = h / sqrt(mean(h^2) + eps) * weight
-// in float32, then the unit's quantisation. `tpr` threads hold a row (one unit
-// each): a power of two up to 32, several rows a CTA, or one row a CTA. The
-// sum of squares goes through 32 values a thread, an xor butterfly over the
-// row's lanes and the warps in order, all in float32, so it does not depend on
-// the launch. Without a weight: y = h.
+// h * w / sqrt(v), rounded to odd: cut off to float32, with the last bit set
+// where something was cut. A second rounding, to a format of at most 22 bits,
+// then gives what rounding the exact value would, so the quantisation that
+// follows sees no float32 tie that is none. inv = hi + lo is 1 / sqrt(v) to some
+// 2^-48; h w is exact as p (16-bit types) or p + e. `cut`: lo is not zero, so
+// that no product is a float32; rows with lo = 0 (1 / sqrt(v) is a float32)
+// look at the remainder.
+template <int kDt>
+__device__ __forceinline__ float mx_norm_value(float h, float w, float hi, float lo, bool cut) {
+  const float p = __fmul_rn(h, w);
+  float t = __fmul_rn(p, lo);
+  if (kDt == kDtFp32) t = fmaf(fmaf(h, w, -p), hi, t);
+  const float y = __fmaf_rz(p, hi, t);
+  if (cut) return __uint_as_float(__float_as_uint(y) | 1u);
+  const bool rest = fmaf(p, hi, -y) != -t;
+  return __uint_as_float(__float_as_uint(y) | (rest ? 1u : 0u));
+}
+
+constexpr int kNormPer = 2;  // spans of a thread
+
+// h = T(residual + x) (written back), y = h / sqrt(mean(h^2) + eps) * weight,
+// then the block's quantisation. `tpr` threads hold a row: a power of two up
+// to 32 (several rows a CTA), or the CTA. Squares are summed eight at a time in
+// float32 and from there on in float64, in an order that depends on the width
+// alone; their sum's error is then far below the float32 steps of y, which
+// decides how often a value lands on the wrong side of a border of the format.
+// Without a weight: y = h.
 template <int kFmt, int kDt, int kMaxT>
 __global__ void __launch_bounds__(kMaxT)
     mx_norm_kernel(const uint8_t* __restrict__ x, int64_t x_ld_bytes, uint8_t* residual, int64_t res_ld_bytes,
-                   const uint8_t* __restrict__ weight, float eps, int64_t rows, uint32_t per_row, uint32_t tpr,
-                   const float* __restrict__ global_scale, uint8_t* __restrict__ q, void* __restrict__ scale) {
-  __shared__ float warp_ss[32];
+                   const uint8_t* __restrict__ weight, bool wide, float eps, int64_t rows, uint32_t per_row,
+                   uint32_t tpr, const float* __restrict__ global_scale, uint8_t* __restrict__ q,
+                   uint8_t* __restrict__ scale) {
+  __shared__ double warp_ss[32];
   griddep_wait();
   griddep_launch_dependents();
   const uint32_t tid = threadIdx.x;
   const bool whole = tpr > 32;  // one row for the CTA
   const int64_t row = whole ? blockIdx.x : blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) + tid / tpr;
-  const uint32_t c = whole ? tid : tid % tpr;
-  const bool live = row < rows && c < per_row;
-  constexpr int kW = MxWords<kDt>::n;
-  float f[32];
-  if (live) {
-    uint32_t w[kW];
-    mx_load<kW>(x + row * x_ld_bytes + static_cast<int64_t>(c) * (4 * kW), w);
-    if (residual) {
-      uint8_t* rp = residual + row * res_ld_bytes + static_cast<int64_t>(c) * (4 * kW);
-      uint32_t rw[kW];
-      mx_load<kW>(rp, rw);
-      float r[32];
-      mx_to_float<kDt>(w, f);
-      mx_to_float<kDt>(rw, r);
+  const uint32_t c0 = whole ? tid : tid % tpr;
+  constexpr int kW = MxWords<kDt, kMxSpan>::n;
+  constexpr int kB = 4 * kW;
+  uint32_t w[kNormPer][kW];
+  bool live[kNormPer];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] += r[i];
-      mx_from_float<kDt>(f, w);
-      mx_store<kW>(rp, w);
+  for (int j = 0; j < kNormPer; ++j) {
+    const uint32_t c = c0 + j * tpr;
+    live[j] = row < rows && c < per_row;
+    if (live[j]) {
+      mx_load<kW>(x + row * x_ld_bytes + static_cast<int64_t>(c) * kB, wide, w[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kW; ++i) w[j][i] = 0;
     }
-    mx_to_float<kDt>(w, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = 0.f;
   }
-  if (weight) {
-    float ss = 0.f;
+  if (residual) {
+    uint8_t* rp = residual + row * res_ld_bytes + static_cast<int64_t>(c0) * kB;
+    uint32_t rw[kNormPer][kW];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) ss = fmaf(f[i], f[i], ss);
+    for (int j = 0; j < kNormPer; ++j)
+      if (live[j]) mx_load<kW>(rp + static_cast<int64_t>(j) * tpr * kB, wide, rw[j]);
+#pragma unroll
+    for (int j = 0; j < kNormPer; ++j) {
+      if (!live[j]) continue;
+      float f[kMxSpan], r[kMxSpan];
+      mx_to_float<kDt>(w[j], f);
+      mx_to_float<kDt>(rw[j], r);
+#pragma unroll
+      for (int i = 0; i < kMxSpan; ++i) f[i] += r[i];
+      mx_from_float<kDt>(f, w[j]);
+      mx_store<kW>(rp + static_cast<int64_t>(j) * tpr * kB, wide, w[j]);
+    }
+  }
+  float hi = 1.f, lo = 0.f;
+  if (weight) {
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < kNormPer; ++j) {
+      float f[kMxSpan];
+      mx_to_float<kDt>(w[j], f);
+#pragma unroll
+      for (int i = 0; i < kMxSpan; i += 8) {
+        float a[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] = fmaf(f[i + 2 * k + 1], f[i + 2 * k + 1], f[i + 2 * k] * f[i + 2 * k]);
+        ss += static_cast<double>((a[0] + a[1]) + (a[2] + a[3]));
+      }
+    }
     for (uint32_t off = whole ? 16 : tpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     if (whole) {
       if ((tid & 31) == 0) warp_ss[tid >> 5] = ss;
       __syncthreads();
-      ss = 0.f;
+      ss = 0.0;
       for (uint32_t i = 0; i < blockDim.x / 32; ++i) ss += warp_ss[i];
     }
-    const float mean = __fdiv_rn(ss, static_cast<float>(per_row * kMxUnit));
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
-    if (live) {
-      uint32_t w[kW];
-      const uint4* wp = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(c) * (4 * kW));
+    const double v = ss / static_cast<double>(per_row * kMxSpan) + static_cast<double>(eps);
+    // 1 / sqrt(v): one Newton step from the float32 estimate (2^-22) where that
+    // is an ordinary number, else the plain operations (zero rows, huge ones)
+    double inv;
+    if (v > 1e-30 && v < 1e30) {
+      const double r = static_cast<double>(rsqrtf(static_cast<float>(v)));
+      inv = fma(r * fma(-v * r, r, 1.0), 0.5, r);
+    } else {
+      inv = 1.0 / sqrt(v);
+    }
+    hi = static_cast<float>(inv);
+    lo = static_cast<float>(inv - static_cast<double>(hi));
+    if (!(fabsf(hi) < INFINITY)) lo = 0.f;
+  }
+  const bool cut = lo != 0.f;
+  const MxGlobal gl = mx_global(kFmt == kFmtNvfp4 ? global_scale : nullptr);
+#pragma unroll
+  for (int j = 0; j < kNormPer; ++j) {
+    const uint32_t c = c0 + j * tpr;
+    float f[kMxSpan];
+    mx_to_float<kDt>(w[j], f);
+    if (weight && live[j]) {
+      uint32_t ww[kW];
+      const uint4* wp = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(c) * kB);
 #pragma unroll
       for (int i = 0; i < kW / 4; ++i) {
         const uint4 v = __ldg(wp + i);
-        w[4 * i] = v.x;
-        w[4 * i + 1] = v.y;
-        w[4 * i + 2] = v.z;
-        w[4 * i + 3] = v.w;
+        ww[4 * i] = v.x;
+        ww[4 * i + 1] = v.y;
+        ww[4 * i + 2] = v.z;
+        ww[4 * i + 3] = v.w;
       }
-      float wf[32];
-      mx_to_float<kDt>(w, wf);
+      float wf[kMxSpan];
+      mx_to_float<kDt>(ww, wf);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = __fmul_rn(__fmul_rn(f[i], inv), wf[i]);
+      for (int i = 0; i < kMxSpan; ++i) f[i] = mx_norm_value<kDt>(f[i], wf[i], hi, lo, cut);
     }
+    const uint32_t am = mx_block_max<kFmt>(mx_span_max(f));
+    uint32_t p[4];
+    const uint32_t sc = mx_quant_span<kFmt>(f, am, gl, p);
+    if (live[j]) mx_store_packed<kFmt>(q, scale, static_cast<uint64_t>(row) * per_row + c, p, sc);
   }
-  if (!live) return;
-  uint32_t am[2];
-  mx_amax<kFmt>(f, am);
-  const float g = (kFmt == kFmtNvfp4 && global_scale) ? __ldg(global_scale) : 1.0f;
-  uint32_t o[8];
-  const uint32_t sc = mx_quant_unit<kFmt>(f, am, g, o);
-  constexpr int kB = mx_unit_bytes(kFmt);
-  const uint64_t u = static_cast<uint64_t>(row) * per_row + c;
-  mx_store<kB / 4>(q + u * kB, o);
-  store_scale(scale, u, mx_unit_scales(kFmt), sc);
 }
 
 constexpr int64_t dt_bytes(int dt) { return dt == kDtFp32 ? 4 : 2; }
 
-// Calls fn<fmt, dt>() for the run-time pair.
+// Calls CALL(fmt, dt) for the run-time pair.
 #define MX_DISPATCH(fmt, dt, CALL)                     \
   switch ((fmt) * 3 + (dt)) {                          \
     case 0: return CALL(kFmtNvfp4, kDtBf16);           \
@@ -197,20 +287,31 @@ constexpr int64_t dt_bytes(int dt) { return dt == kDtFp32 ? 4 : 2; }
     default: return CALL(kFmtMxfp8, kDtFp32);          \
   }
 
+bool wide_rows(const void* p, int64_t ld_bytes) {
+  return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld_bytes)) & 31u) == 0;
+}
+
+dim3 mx_grid(uint64_t pieces, int per) {
+  return dim3(static_cast<uint32_t>((pieces + kMxThreads * per - 1) / (kMxThreads * per)));
+}
+
 template <int kFmt, int kDt>
 cudaError_t norm_launch(const MxNormCall& c, cudaStream_t s) {
-  const uint32_t per_row = static_cast<uint32_t>(c.cols / kMxUnit);
-  uint32_t tpr = 1;
+  const uint32_t per_row = static_cast<uint32_t>(c.cols / kMxSpan);
+  // up to two spans a thread: narrow rows share a CTA of 128 threads
+  uint32_t tpr = 2;
   while (tpr < per_row && tpr < 32) tpr *= 2;
-  const bool whole = per_row > 32;
-  const uint32_t threads = whole ? (per_row + 31) / 32 * 32 : 128;
-  if (whole) tpr = threads;
-  const int64_t grid = whole ? c.rows : (c.rows + 128 / tpr - 1) / (128 / tpr);
+  uint32_t threads = 128;
+  const bool whole = per_row > 32 * kNormPer;
+  if (whole) tpr = threads = (per_row + 32 * kNormPer - 1) / (32 * kNormPer) * 32;
+  const int64_t grid = whole ? c.rows : (c.rows + threads / tpr - 1) / (threads / tpr);
+  const int64_t x_ld = c.x_ld * dt_bytes(kDt), res_ld = c.res_ld * dt_bytes(kDt);
+  const bool wide = wide_rows(c.x, x_ld) && wide_rows(c.residual, c.residual ? res_ld : 0);
   auto go = [&](auto kernel) {
     return launch_k(kernel, dim3(static_cast<uint32_t>(grid)), dim3(threads), 0, s, true,
-                    static_cast<const uint8_t*>(c.x), c.x_ld * dt_bytes(kDt), static_cast<uint8_t*>(c.residual),
-                    c.res_ld * dt_bytes(kDt), static_cast<const uint8_t*>(c.weight), c.eps, c.rows, per_row, tpr,
-                    c.global_scale, static_cast<uint8_t*>(c.q), c.scale);
+                    static_cast<const uint8_t*>(c.x), x_ld, static_cast<uint8_t*>(c.residual), res_ld,
+                    static_cast<const uint8_t*>(c.weight), wide, c.eps, c.rows, per_row, tpr, c.global_scale,
+                    static_cast<uint8_t*>(c.q), static_cast<uint8_t*>(c.scale));
   };
   // rows of up to 8192 columns keep a bound that leaves the compiler 255 registers
   if (threads <= 256) return go(mx_norm_kernel<kFmt, kDt, 256>);
@@ -221,26 +322,26 @@ cudaError_t norm_launch(const MxNormCall& c, cudaStream_t s) {
 
 cudaError_t launch_mx_quant(const void* x, int dt, int64_t x_ld, int64_t rows, int64_t cols, int fmt,
                             const float* global_scale, void* q, void* scale, cudaStream_t s) {
-  const uint32_t per_row = static_cast<uint32_t>(cols / kMxUnit);
-  const uint64_t units = static_cast<uint64_t>(rows) * per_row;
-  if (units == 0) return cudaSuccess;
-  const dim3 grid(static_cast<uint32_t>((units + kMxThreads - 1) / kMxThreads));
-#define CALL(F, D)                                                                                              \
-  launch_k(mx_quant_kernel<F, D>, grid, dim3(kMxThreads), 0, s, true, static_cast<const uint8_t*>(x),           \
-           x_ld * dt_bytes(D), units, per_row, global_scale, static_cast<uint8_t*>(q), scale)
+  const uint32_t per_row = static_cast<uint32_t>(cols / kMxSpan);
+  const uint64_t spans = static_cast<uint64_t>(rows) * per_row;
+  if (spans == 0) return cudaSuccess;
+#define CALL(F, D)                                                                                                    \
+  launch_k(mx_quant_kernel<F, D>, mx_grid(spans, kQuantPer), dim3(kMxThreads), 0, s, true, static_cast<const uint8_t*>(x), \
+           x_ld * dt_bytes(D), wide_rows(x, x_ld * dt_bytes(D)), spans, per_row, global_scale,                       \
+           static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale))
   MX_DISPATCH(fmt, dt, CALL)
 #undef CALL
 }
 
 cudaError_t launch_mx_dequant(const void* q, const void* scale, int64_t rows, int64_t cols, int fmt,
                               const float* global_scale, int dt, void* x, int64_t x_ld, cudaStream_t s) {
-  const uint32_t per_row = static_cast<uint32_t>(cols / kMxUnit);
-  const uint64_t units = static_cast<uint64_t>(rows) * per_row;
-  if (units == 0) return cudaSuccess;
-  const dim3 grid(static_cast<uint32_t>((units + kMxThreads - 1) / kMxThreads));
-#define CALL(F, D)                                                                                              \
-  launch_k(mx_dequant_kernel<F, D>, grid, dim3(kMxThreads), 0, s, true, static_cast<const uint8_t*>(q), scale, units, \
-           per_row, global_scale, static_cast<uint8_t*>(x), x_ld * dt_bytes(D))
+  const uint32_t per_row = static_cast<uint32_t>(cols / kMxOctet);
+  const uint64_t octets = static_cast<uint64_t>(rows) * per_row;
+  if (octets == 0) return cudaSuccess;
+#define CALL(F, D)                                                                                                      \
+  launch_k(mx_dequant_kernel<F, D>, mx_grid(octets, kDequantPer), dim3(kMxThreads), 0, s, true, static_cast<const uint8_t*>(q), \
+           static_cast<const uint8_t*>(scale), octets, per_row, global_scale, static_cast<uint8_t*>(x),                 \
+           x_ld * dt_bytes(D), wide_rows(x, x_ld * dt_bytes(D)))
   MX_DISPATCH(fmt, dt, CALL)
 #undef CALL
 }

@@ -24,8 +24,9 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .binding import _call, _need, _stream
+from .binding import _stream
 
+_Tensor = torch.Tensor
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
 
@@ -42,77 +43,128 @@ MAX_N = 1 << 18
 MAX_EXPERTS = 512
 MAX_NORM_COLS = 32768
 
+# The checks below build their messages only when they fail: these calls are
+# short, and formatting took longer than the kernels of a decode step.
+
+
+def _bad(msg):
+    raise ValueError(msg)
+
+
+def _run(dev, name, *args):
+    """Calls a C-ABI function with `dev` current on its current stream."""
+    fn = getattr(_lib._lib or _lib.load(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        _lib.check(rc, name)
+
 
 def _format(fmt):
     f = _FORMATS.get(fmt) if isinstance(fmt, str) else None
-    _need(f is not None, f"fmt must be one of {sorted(_FORMATS)}, got {fmt!r}")
-    return f
+    return f or _bad(f"fmt must be one of {sorted(_FORMATS)}, got {fmt!r}")
 
 
-def _is(t, name):
-    _need(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
-    _need(t.is_cuda, f"{name} must be a CUDA tensor")
+def _cuda(t, name):
+    if not isinstance(t, _Tensor):
+        _bad(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        _bad(f"{name} must be a CUDA tensor")
+    return t.device
 
 
-def _matrix(t, name, dev=None, dtype=None, shape=None):
-    """A 2-D bf16, fp16 or fp32 CUDA tensor whose rows are contiguous and
-    16-byte aligned (any row stride); returns its dtype code."""
-    _is(t, name)
-    _need(t.dim() == 2, f"{name} must be 2-D, got {t.dim()}-D")
+def _matrix(t, name, dev, dtype=None, shape=None):
+    """A 2-D bf16, fp16 or fp32 tensor on `dev` whose rows are contiguous and
+    16-byte aligned (any row stride); returns (dtype code, row stride)."""
+    if not isinstance(t, _Tensor) or t.device != dev:
+        _cuda(t, name)
+        _bad(f"{name} must be on {dev}")
     code = _DTYPES.get(t.dtype)
-    _need(code is not None, f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if dtype is not None:
-        _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None:
-        _need(tuple(t.shape) == shape, f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if dev is not None:
-        _need(t.device == dev, f"{name} must be on {dev}")
-    if t.numel():
-        rows, cols = t.shape
-        _need(cols == 1 or t.stride(1) == 1, f"{name}'s rows must be contiguous")
-        _need(rows == 1 or t.stride(0) >= cols, f"{name}'s rows must not overlap")
-        size = t.element_size()
-        _need(t.data_ptr() % 16 == 0 and (rows == 1 or t.stride(0) * size % 16 == 0),
-              f"{name}'s rows must be 16-byte aligned")
-    return code
+    if code is None:
+        _bad(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        _bad(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2:
+        _bad(f"{name} must be 2-D, got {t.dim()}-D")
+    rows, cols = t.shape
+    if shape is not None and (rows, cols) != shape:
+        _bad(f"{name} must have shape {shape}, got {(rows, cols)}")
+    ld, inner = t.stride()
+    if rows and cols:
+        if inner != 1 and cols != 1:
+            _bad(f"{name}'s rows must be contiguous")
+        if rows == 1:
+            ld = cols
+        elif ld < cols:
+            _bad(f"{name}'s rows must not overlap")
+        if t.data_ptr() % 16 or (rows > 1 and ld * (4 if code == 2 else 2) % 16):
+            _bad(f"{name}'s rows must be 16-byte aligned")
+    return code, ld
 
 
 def _exact(t, name, dtype, shape, dev):
     """A contiguous tensor of the given type, shape and device."""
-    _is(t, name)
-    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _need(tuple(t.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    _need(t.device == dev, f"{name} must be on {dev}")
-    _need(t.is_contiguous(), f"{name} must be contiguous")
-
-
-def _scalar(t, name, dev, fmt=None):
-    if t is None:
-        return None
-    _need(fmt is None or fmt == "nvfp4", f"{name} belongs to nvfp4, not to {fmt}")
-    _is(t, name)
-    _need(t.dtype == torch.float32 and t.numel() == 1, f"{name} must be a float32 tensor of one element")
-    _need(t.device == dev, f"{name} must be on {dev}")
+    if (not isinstance(t, _Tensor) or t.dtype != dtype or t.shape != shape or t.device != dev
+            or not t.is_contiguous()):
+        _cuda(t, name)
+        if t.dtype != dtype:
+            _bad(f"{name} must be {dtype}, got {t.dtype}")
+        if t.shape != shape:
+            _bad(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.device != dev:
+            _bad(f"{name} must be on {dev}")
+        _bad(f"{name} must be contiguous")
     return t.data_ptr()
 
 
-def _width(cols, limit=MAX_COLS):
-    _need(0 < cols <= limit and cols % 32 == 0, f"the width must be a multiple of 32 in 32..{limit}, got {cols}")
+def _exact16(t, name, dtype, shape, dev):
+    p = _exact(t, name, dtype, shape, dev)
+    if p % 16:
+        _bad(f"{name} must be 16-byte aligned")
+    return p
+
+
+def _scalar(t, name, dev):
+    """Address of a float32 tensor of one element, or None."""
+    if t is None:
+        return None
+    if not isinstance(t, _Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != dev:
+        _cuda(t, name)
+        if t.device != dev:
+            _bad(f"{name} must be on {dev}")
+        _bad(f"{name} must be a float32 tensor of one element")
+    return t.data_ptr()
+
+
+def _global_scale(t, fmt, dev):
+    if t is not None and fmt != "nvfp4":
+        _bad(f"global_scale belongs to nvfp4, not to {fmt}")
+    return _scalar(t, "global_scale", dev)
+
+
+def _size(rows, cols, limit=MAX_COLS):
+    if cols % 32 or not 0 < cols <= limit:
+        _bad(f"the width must be a multiple of 32 in 32..{limit}, got {cols}")
+    if rows > MAX_ROWS:
+        _bad(f"at most {MAX_ROWS} rows, got {rows}")
 
 
 def _packed_out(rows, cols, f, dev, out, out_scale):
     _, qt, per, st, block = f
     if out is None:
         out = torch.empty((rows, cols // per), dtype=qt, device=dev)
+        qp = out.data_ptr()
     else:
-        _exact(out, "out", qt, (rows, cols // per), dev)
-        _need(out.data_ptr() % 16 == 0, "out must be 16-byte aligned")
+        qp = _exact16(out, "out", qt, (rows, cols // per), dev)
     if out_scale is None:
         out_scale = torch.empty((rows, cols // block), dtype=st, device=dev)
+        sp = out_scale.data_ptr()
     else:
-        _exact(out_scale, "out_scale", st, (rows, cols // block), dev)
-        _need(out_scale.data_ptr() % 2 == 0 or block != 16, "out_scale must be 2-byte aligned")
-    return out, out_scale
+        sp = _exact(out_scale, "out_scale", st, (rows, cols // block), dev)
+    return out, out_scale, qp, sp
 
 
 def quantize_mx(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | None = None,
@@ -129,32 +181,27 @@ def quantize_mx(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor 
     A block with an infinity or a NaN gets a NaN scale (its values read back
     as NaN) and zeros."""
     f = _format(fmt)
-    code = _matrix(x, "x")
+    dev = _cuda(x, "x")
+    code, ld = _matrix(x, "x", dev)
     rows, cols = x.shape
-    _width(cols)
-    _need(rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
-    dev = x.device
-    g = _scalar(global_scale, "global_scale", dev, fmt)
-    out, out_scale = _packed_out(rows, cols, f, dev, out, out_scale)
+    _size(rows, cols)
+    g = _global_scale(global_scale, fmt, dev)
+    out, out_scale, qp, sp = _packed_out(rows, cols, f, dev, out, out_scale)
     if rows:
-        rc = _call(dev, _lib.load().moe_fp8_ds_quantize_mx, x.data_ptr(), code, rows, cols, x.stride(0), f[0], g,
-                   out.data_ptr(), out_scale.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_quantize_mx")
+        _run(dev, "moe_fp8_ds_quantize_mx", x.data_ptr(), code, rows, cols, ld, f[0], g, qp, sp)
     return out, out_scale
 
 
 def _packed_in(q, scale, f, dev, names, lead=()):
-    """Checks packed data and its scales (leading dims `lead`); returns (rows, cols)."""
+    """Checks packed data and its scales (leading dims `lead`); returns (rows, cols, addresses)."""
     _, qt, per, st, block = f
-    _is(q, names[0])
-    _need(q.dim() == 2 + len(lead), f"{names[0]} must be {2 + len(lead)}-D, got {q.dim()}-D")
+    if not isinstance(q, _Tensor) or q.dim() != 2 + len(lead):
+        _cuda(q, names[0])
+        _bad(f"{names[0]} must be {2 + len(lead)}-D, got {q.dim()}-D")
     rows, cols = q.shape[-2], q.shape[-1] * per
-    _width(cols)
-    _exact(q, names[0], qt, (*lead, rows, cols // per), dev)
-    _exact(scale, names[1], st, (*lead, rows, cols // block), dev)
-    _need(q.data_ptr() % 16 == 0, f"{names[0]} must be 16-byte aligned")
-    return rows, cols
+    _size(rows, cols)
+    qp = _exact16(q, names[0], qt, (*lead, rows, cols // per), dev)
+    return rows, cols, qp, _exact(scale, names[1], st, (*lead, rows, cols // block), dev)
 
 
 def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | None = None,
@@ -162,21 +209,18 @@ def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, fmt: str = "nvfp4", glob
     """The values that packed data stands for, [rows, cols]: value * scale *
     global_scale in float32, rounded once to ``dtype`` (bf16, fp16 or fp32)."""
     f = _format(fmt)
-    _is(q, "q")
-    dev = q.device
-    rows, cols = _packed_in(q, scale, f, dev, ("q", "scale"))
-    _need(rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
-    _need(f[4] != 16 or scale.data_ptr() % 2 == 0, "scale must be 2-byte aligned")
-    g = _scalar(global_scale, "global_scale", dev, fmt)
+    dev = _cuda(q, "q")
+    rows, cols, qp, sp = _packed_in(q, scale, f, dev, ("q", "scale"))
+    g = _global_scale(global_scale, fmt, dev)
     if out is None:
-        _need(dtype in _DTYPES, f"dtype must be bfloat16, float16 or float32, got {dtype}")
+        code, ld = _DTYPES.get(dtype), cols
+        if code is None:
+            _bad(f"dtype must be bfloat16, float16 or float32, got {dtype}")
         out = torch.empty((rows, cols), dtype=dtype, device=dev)
-    code = _matrix(out, "out", dev, None, (rows, cols))
+    else:
+        code, ld = _matrix(out, "out", dev, None, (rows, cols))
     if rows:
-        rc = _call(dev, _lib.load().moe_fp8_ds_dequantize_mx, q.data_ptr(), scale.data_ptr(), rows, cols, f[0], g, code,
-                   out.data_ptr(), out.stride(0), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_dequantize_mx")
+        _run(dev, "moe_fp8_ds_dequantize_mx", qp, sp, rows, cols, f[0], g, code, out.data_ptr(), ld)
     return out
 
 
@@ -186,45 +230,57 @@ def add_rmsnorm_quantize_mx(x: torch.Tensor, residual: torch.Tensor | None = Non
                             out_scale: torch.Tensor | None = None):
     """``add_rmsnorm_quantize`` for any width up to 32768 and for the
     microscaled formats: ``h = residual + x`` rounded to x's type (written back
-    into ``residual``), ``y = h / sqrt(mean(h^2) + eps) * norm_weight`` in
-    float32, then the quantisation of y as in ``quantize_mx``. ``residual``
-    None: h = x; ``norm_weight`` None: y = h. All three tensors have x's type.
-    Returns (packed values, scales)."""
+    into ``residual``), ``y = h / sqrt(mean(h^2) + eps) * norm_weight``, then
+    the quantisation of y as in ``quantize_mx`` (y is rounded to odd in float32,
+    so a value lands where the exact y would). ``residual`` None: h = x;
+    ``norm_weight`` None: y = h. All three tensors have x's type. Returns
+    (packed values, scales)."""
     f = _format(fmt)
-    code = _matrix(x, "x")
-    rows, cols = x.shape
-    _width(cols, MAX_NORM_COLS)
-    _need(rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
-    _need(float(eps) >= 0.0, "eps must be >= 0")
-    dev = x.device
+    dev = _cuda(x, "x")
+    code, ld = _matrix(x, "x", dev)
+    rows, cols = shape = x.shape
+    _size(rows, cols, MAX_NORM_COLS)
+    eps = float(eps)
+    if not eps >= 0.0:
+        _bad("eps must be >= 0")
+    rp, rld, wp = None, 0, None
     if residual is not None:
-        _matrix(residual, "residual", dev, x.dtype, (rows, cols))
+        rld = _matrix(residual, "residual", dev, x.dtype, shape)[1]
+        rp = residual.data_ptr()
     if norm_weight is not None:
-        _exact(norm_weight, "norm_weight", x.dtype, (cols,), dev)
-        _need(norm_weight.data_ptr() % 16 == 0, "norm_weight must be 16-byte aligned")
-    g = _scalar(global_scale, "global_scale", dev, fmt)
-    out, out_scale = _packed_out(rows, cols, f, dev, out, out_scale)
+        wp = _exact16(norm_weight, "norm_weight", x.dtype, (cols,), dev)
+    g = _global_scale(global_scale, fmt, dev)
+    out, out_scale, qp, sp = _packed_out(rows, cols, f, dev, out, out_scale)
     if rows:
-        rc = _call(dev, _lib.load().moe_fp8_ds_add_norm_quantize_mx, x.data_ptr(), x.stride(0),
-                   None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-                   None if norm_weight is None else norm_weight.data_ptr(), float(eps), code, rows, cols, f[0], g,
-                   out.data_ptr(), out_scale.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_add_norm_quantize_mx")
+        _run(dev, "moe_fp8_ds_add_norm_quantize_mx", x.data_ptr(), ld, rp, rld, wp, eps, code, rows, cols, f[0], g, qp, sp)
     return out, out_scale
 
 
 def _product_out(m, n, dev, out, out_dtype, make):
     if out is None:
-        _need(out_dtype in _DTYPES, f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-        return make((m, n), dtype=out_dtype, device=dev), _DTYPES[out_dtype]
-    _is(out, "out")
+        code = _DTYPES.get(out_dtype)
+        if code is None:
+            _bad(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+        return make((m, n), dtype=out_dtype, device=dev), code, n
+    if not isinstance(out, _Tensor) or out.device != dev:
+        _cuda(out, "out")
+        _bad(f"out must be on {dev}")
     code = _DTYPES.get(out.dtype)
-    _need(code is not None, f"out must be bfloat16, float16 or float32, got {out.dtype}")
-    _need(tuple(out.shape) == (m, n), f"out must have shape {(m, n)}, got {tuple(out.shape)}")
-    _need(out.device == dev, f"out must be on {dev}")
-    _need(m == 0 or ((n == 1 or out.stride(1) == 1) and (m == 1 or out.stride(0) >= n)), "out's rows must be contiguous")
-    return out, code
+    if code is None:
+        _bad(f"out must be bfloat16, float16 or float32, got {out.dtype}")
+    if out.shape != (m, n):
+        _bad(f"out must have shape {(m, n)}, got {tuple(out.shape)}")
+    ld, inner = out.stride()
+    if m and ((inner != 1 and n != 1) or (m > 1 and ld < n)):
+        _bad("out's rows must be contiguous")
+    return out, code, ld if m > 1 else n
+
+
+def _same_width(k, kb, m, n):
+    if k != kb:
+        _bad(f"a and b must have the same width, got {k} and {kb}")
+    if not 0 < n <= MAX_N:
+        _bad(f"b must have 1..{MAX_N} rows, got {n}")
 
 
 def matmul_mx(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, fmt: str = "nvfp4",
@@ -237,19 +293,14 @@ def matmul_mx(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     element, for nvfp4 the product of the two global scales; None = 1. e4m3
     scales must not be negative."""
     f = _format(fmt)
-    _is(a, "a")
-    dev = a.device
-    m, k = _packed_in(a, a_scale, f, dev, ("a", "a_scale"))
-    n, kb = _packed_in(b, b_scale, f, dev, ("b", "b_scale"))
-    _need(k == kb, f"a and b must have the same width, got {k} and {kb}")
-    _need(m <= MAX_ROWS and 0 < n <= MAX_N, f"a has at most {MAX_ROWS} rows and b 1..{MAX_N}")
+    dev = _cuda(a, "a")
+    m, k, ap, asp = _packed_in(a, a_scale, f, dev, ("a", "a_scale"))
+    n, kb, bp, bsp = _packed_in(b, b_scale, f, dev, ("b", "b_scale"))
+    _same_width(k, kb, m, n)
     al = _scalar(alpha, "alpha", dev)
-    out, code = _product_out(m, n, dev, out, out_dtype, torch.empty)
+    out, code, ld = _product_out(m, n, dev, out, out_dtype, torch.empty)
     if m:
-        rc = _call(dev, _lib.load().moe_fp8_ds_matmul_mx, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
-                   b_scale.data_ptr(), m, n, k, f[0], al, out.data_ptr(), code, out.stride(0), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_matmul_mx")
+        _run(dev, "moe_fp8_ds_matmul_mx", ap, asp, bp, bsp, m, n, k, f[0], al, out.data_ptr(), code, ld)
     return out
 
 
@@ -264,24 +315,19 @@ def experts_matmul_mx(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b
     copied to the host. Rows outside the runs are left as they were (zero where
     ``out`` is None)."""
     f = _format(fmt)
-    _is(a, "a")
-    _is(b, "b")
-    dev = a.device
-    m, k = _packed_in(a, a_scale, f, dev, ("a", "a_scale"))
-    _need(b.dim() == 3, f"b must be 3-D, got {b.dim()}-D")
+    dev = _cuda(a, "a")
+    m, k, ap, asp = _packed_in(a, a_scale, f, dev, ("a", "a_scale"))
+    _cuda(b, "b")
+    if b.dim() != 3:
+        _bad(f"b must be 3-D, got {b.dim()}-D")
     e = b.shape[0]
-    _need(1 <= e <= MAX_EXPERTS, f"b must hold 1..{MAX_EXPERTS} experts, got {e}")
-    n, kb = _packed_in(b, b_scale, f, dev, ("b", "b_scale"), (e,))
-    _need(k == kb, f"a and b must have the same width, got {k} and {kb}")
-    _need(m <= MAX_ROWS and 0 < n <= MAX_N, f"a has at most {MAX_ROWS} rows and b 1..{MAX_N}")
-    _exact(expert_offsets, "expert_offsets", torch.int32, (e + 1,), dev)
-    if alpha is not None:
-        _exact(alpha, "alpha", torch.float32, (e,), dev)
-    out, code = _product_out(m, n, dev, out, out_dtype, torch.zeros)
+    if not 1 <= e <= MAX_EXPERTS:
+        _bad(f"b must hold 1..{MAX_EXPERTS} experts, got {e}")
+    n, kb, bp, bsp = _packed_in(b, b_scale, f, dev, ("b", "b_scale"), (e,))
+    _same_width(k, kb, m, n)
+    op = _exact(expert_offsets, "expert_offsets", torch.int32, (e + 1,), dev)
+    al = None if alpha is None else _exact(alpha, "alpha", torch.float32, (e,), dev)
+    out, code, ld = _product_out(m, n, dev, out, out_dtype, torch.zeros)
     if m:
-        rc = _call(dev, _lib.load().moe_fp8_ds_experts_matmul_mx, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
-                   b_scale.data_ptr(), expert_offsets.data_ptr(), e, m, n, k, f[0],
-                   None if alpha is None else alpha.data_ptr(), out.data_ptr(), code, out.stride(0), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_experts_matmul_mx")
+        _run(dev, "moe_fp8_ds_experts_matmul_mx", ap, asp, bp, bsp, op, e, m, n, k, f[0], al, out.data_ptr(), code, ld)
     return out

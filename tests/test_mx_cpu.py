@@ -45,7 +45,7 @@ def _dequant(lib, **k):
 BAD_ROWS = [(dict(rows=-1), INVALID), (dict(rows=(1 << 24) + 1), INVALID), (dict(cols=0), INVALID), (dict(cols=48), INVALID),
             (dict(cols=1 << 21, ld=1 << 21), INVALID), (dict(fmt=3), INVALID), (dict(fmt=-1), INVALID), (dict(dt=3), INVALID),
             (dict(x=None), INVALID), (dict(q=None), INVALID), (dict(s=None), INVALID), (dict(ld=32), INVALID),
-            (dict(fmt=1, g=P), INVALID), (dict(x=P + 8), ALIGN), (dict(q=P + 8), ALIGN), (dict(s=P + 1), ALIGN),
+            (dict(fmt=1, g=P), INVALID), (dict(x=P + 8), ALIGN), (dict(q=P + 8), ALIGN),
             (dict(ld=68), ALIGN), (dict(g=P + 2), ALIGN)]
 
 
