@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .binding import _call, _need, _stream
+from .mx import _bad, _cuda, _run
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SCORES = {"sigmoid": 0, "softmax": 1}
@@ -20,42 +20,42 @@ MAX_TOKENS = 1 << 24
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, offsets, coeff, score):
-        T, E = logits.shape
-        S = 1 if offsets is None else offsets.shape[0] - 1
-        dev = logits.device
-        lib = _lib.load()
-        work = torch.empty(lib.moe_fp8_ds_balance_loss_work_bytes(T, E, S), dtype=torch.uint8, device=dev)
-        loss = torch.empty(S, dtype=torch.float32, device=dev)
-        counts = torch.empty((S, E), dtype=torch.int32, device=dev)
-        off = None if offsets is None else offsets.data_ptr()
-        rc = _call(dev, lib.moe_fp8_ds_balance_loss, logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0),
-                   ids.data_ptr(), off, T, E, ids.shape[1], S, score, coeff, work.data_ptr(), loss.data_ptr(),
-                   counts.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_balance_loss")
+        loss, counts = _forward(logits, ids, offsets, coeff, score)
         ctx.save_for_backward(logits, ids, offsets, counts)
-        ctx.coeff, ctx.score = coeff, score
+        ctx.args = coeff, score
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
         if grad_loss is None:
             return None, None, None, None, None
+        if torch.is_grad_enabled():  # create_graph: the gradient's own gradient is not there
+            raise RuntimeError("balance_loss can be differentiated once only")
         logits, ids, offsets, counts = ctx.saved_tensors
+        coeff, score = ctx.args
         T, E = logits.shape
         dev = logits.device
         grad_loss = grad_loss.contiguous()
         grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
-        off = None if offsets is None else offsets.data_ptr()
-        rc = _call(dev, _lib.load().moe_fp8_ds_balance_loss_backward, logits.data_ptr(), _DTYPES[logits.dtype],
-                   logits.stride(0), ids.data_ptr(), off, T, E, ids.shape[1], counts.shape[0], ctx.score, ctx.coeff,
-                   counts.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "moe_fp8_ds_balance_loss_backward")
+        _run(dev, "moe_fp8_ds_balance_loss_backward", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0),
+             ids.data_ptr(), None if offsets is None else offsets.data_ptr(), T, E, ids.shape[1], counts.shape[0], score,
+             coeff, counts.data_ptr(), grad_loss.data_ptr(), grad.data_ptr())
         return grad, None, None, None, None
+
+
+def _forward(logits, ids, offsets, coeff, score):
+    T, E = logits.shape
+    S = 1 if offsets is None else offsets.shape[0] - 1
+    dev = logits.device
+    work = torch.empty(_lib.load().moe_fp8_ds_balance_loss_work_bytes(T, E, S), dtype=torch.uint8, device=dev)
+    loss = torch.empty(S, dtype=torch.float32, device=dev)
+    counts = torch.empty((S, E), dtype=torch.int32, device=dev)
+    _run(dev, "moe_fp8_ds_balance_loss", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), ids.data_ptr(),
+         None if offsets is None else offsets.data_ptr(), T, E, ids.shape[1], S, score, coeff, work.data_ptr(),
+         loss.data_ptr(), counts.data_ptr())
+    return loss, counts
 
 
 def balance_loss(routing_logits: torch.Tensor, topk_ids: torch.Tensor, seq_offsets: torch.Tensor | None = None,
@@ -78,25 +78,37 @@ def balance_loss(routing_logits: torch.Tensor, topk_ids: torch.Tensor, seq_offse
     0; tokens of no sequence count nowhere and get a zero gradient; a token
     whose scores sum to zero in float32 has p = 0. ``counts.sum(0)`` is what a
     bias update of the no-aux router needs."""
-    _need(isinstance(routing_logits, torch.Tensor) and routing_logits.is_cuda, "routing_logits must be a CUDA tensor")
-    _need(isinstance(topk_ids, torch.Tensor) and topk_ids.is_cuda, "topk_ids must be a CUDA tensor")
-    _need(routing_logits.dim() == 2 and topk_ids.dim() == 2, "routing_logits and topk_ids must be 2-D")
-    _need(routing_logits.dtype in _DTYPES, f"routing_logits must be float32, bfloat16 or float16, got {routing_logits.dtype}")
+    dev = _cuda(routing_logits, "routing_logits")
+    _cuda(topk_ids, "topk_ids")
+    if routing_logits.dim() != 2 or topk_ids.dim() != 2:
+        _bad("routing_logits and topk_ids must be 2-D")
+    if routing_logits.dtype not in _DTYPES:
+        _bad(f"routing_logits must be float32, bfloat16 or float16, got {routing_logits.dtype}")
     T, E = routing_logits.shape
-    _need(1 <= E <= MAX_EXPERTS, f"1..{MAX_EXPERTS} experts, got {E}")
-    _need(T <= MAX_TOKENS, f"at most {MAX_TOKENS} tokens")
-    dev = routing_logits.device
-    _need(topk_ids.dtype == torch.int32 and topk_ids.shape[0] == T and 1 <= topk_ids.shape[1] <= E,
-          f"topk_ids must be int32 [{T}, 1..{E}], got {topk_ids.dtype} {tuple(topk_ids.shape)}")
-    _need(topk_ids.device == dev, f"topk_ids must be on {dev}")
-    _need(topk_ids.is_contiguous(), "topk_ids must be contiguous")
-    _need(T == 0 or ((E == 1 or routing_logits.stride(1) == 1) and (T == 1 or routing_logits.stride(0) >= E)),
-          "routing_logits' rows must be contiguous")
-    _need(score_func in _SCORES, f"score_func must be one of {sorted(_SCORES)}, got {score_func!r}")
+    if not 1 <= E <= MAX_EXPERTS:
+        _bad(f"1..{MAX_EXPERTS} experts, got {E}")
+    if T > MAX_TOKENS:
+        _bad(f"at most {MAX_TOKENS} tokens, got {T}")
+    if topk_ids.dtype != torch.int32 or topk_ids.shape[0] != T or not 1 <= topk_ids.shape[1] <= E:
+        _bad(f"topk_ids must be int32 [{T}, 1..{E}], got {topk_ids.dtype} {tuple(topk_ids.shape)}")
+    if topk_ids.device != dev:
+        _bad(f"topk_ids must be on {dev}")
+    if not topk_ids.is_contiguous():
+        _bad("topk_ids must be contiguous")
+    ld, inner = routing_logits.stride()
+    if T and ((inner != 1 and E != 1) or (T > 1 and ld < E)):
+        _bad("routing_logits' rows must be contiguous")
+    score = _SCORES.get(score_func)
+    if score is None:
+        _bad(f"score_func must be one of {sorted(_SCORES)}, got {score_func!r}")
     if seq_offsets is not None:
-        _need(isinstance(seq_offsets, torch.Tensor) and seq_offsets.dtype == torch.int32 and seq_offsets.dim() == 1
-              and seq_offsets.shape[0] >= 2, "seq_offsets must be int32 [sequences + 1]")
-        _need(seq_offsets.device == dev, f"seq_offsets must be on {dev}")
-        _need(seq_offsets.is_contiguous(), "seq_offsets must be contiguous")
-        _need(seq_offsets.shape[0] <= MAX_TOKENS, f"fewer than {MAX_TOKENS} sequences")
-    return _BalanceLoss.apply(routing_logits, topk_ids, seq_offsets, float(coeff), _SCORES[score_func])
+        _cuda(seq_offsets, "seq_offsets")
+        if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or not 2 <= seq_offsets.shape[0] <= MAX_TOKENS:
+            _bad(f"seq_offsets must be int32 [sequences + 1], got {seq_offsets.dtype} {tuple(seq_offsets.shape)}")
+        if seq_offsets.device != dev:
+            _bad(f"seq_offsets must be on {dev}")
+        if not seq_offsets.is_contiguous():
+            _bad("seq_offsets must be contiguous")
+    if routing_logits.requires_grad and torch.is_grad_enabled():
+        return _BalanceLoss.apply(routing_logits, topk_ids, seq_offsets, float(coeff), score)
+    return _forward(routing_logits, topk_ids, seq_offsets, float(coeff), score)

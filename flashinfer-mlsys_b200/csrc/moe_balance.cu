@@ -25,34 +25,72 @@ namespace moe {
 
 namespace {
 
-constexpr int kBalWarps = 8;
+constexpr int kBalWarps = 16;
 constexpr int kBalThreads = kBalWarps * 32;
+// Rows a warp has in flight, for `n` columns a lane (more registers than there are beyond that).
+__host__ __device__ constexpr int bal_batch(int n) { return n >= 32 ? 1 : 4; }
 
-template <int kDt>
-__device__ __forceinline__ float bal_load(const void* row, int c) {
-  if constexpr (kDt == 0) return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[c]);
-  if constexpr (kDt == 1) return __half2float(static_cast<const __half*>(row)[c]);
-  return static_cast<const float*>(row)[c];
+// Columns of a lane: kV neighbours, every 32 kV (kV = 4 where the rows allow
+// vector loads, else 1).
+template <int kDt, int kV>
+__device__ __forceinline__ void bal_load(const void* row, int c, float* v) {
+  if constexpr (kV == 1) {
+    if constexpr (kDt == 0) v[0] = __bfloat162float(static_cast<const __nv_bfloat16*>(row)[c]);
+    if constexpr (kDt == 1) v[0] = __half2float(static_cast<const __half*>(row)[c]);
+    if constexpr (kDt == 2) v[0] = static_cast<const float*>(row)[c];
+  } else if constexpr (kDt == 2) {
+    const float4 t = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + c);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+  } else {
+    const uint2 t = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + c);
+    const uint32_t w[2] = {t.x, t.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = kDt == 0 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]))
+                                : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
 }
-template <int kDt>
-__device__ __forceinline__ void bal_store(void* row, int c, float v) {
-  if constexpr (kDt == 0)
-    static_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(v);
-  else if constexpr (kDt == 1)
-    static_cast<__half*>(row)[c] = __float2half_rn(v);
-  else
-    static_cast<float*>(row)[c] = v;
+template <int kDt, int kV>
+__device__ __forceinline__ void bal_store(void* row, int c, const float* v) {
+  if constexpr (kV == 1) {
+    if constexpr (kDt == 0) static_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(v[0]);
+    if constexpr (kDt == 1) static_cast<__half*>(row)[c] = __float2half_rn(v[0]);
+    if constexpr (kDt == 2) static_cast<float*>(row)[c] = v[0];
+  } else if constexpr (kDt == 2) {
+    *reinterpret_cast<float4*>(static_cast<float*>(row) + c) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (kDt == 0) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&t);
+      } else {
+        const __half2 t = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&t);
+      }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(row) + c) = make_uint2(w[0], w[1]);
+  }
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Sums (maxima) over the warp of several rows at once: their shuffles overlap.
+template <int kB>
+__device__ __forceinline__ void warp_sums(float (&v)[kB]) {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int o = 16; o >= 1; o >>= 1)
+#pragma unroll
+    for (int b = 0; b < kB; ++b) v[b] += __shfl_xor_sync(0xffffffffu, v[b], o);
 }
-__device__ __forceinline__ float warp_max(float v) {
+template <int kB>
+__device__ __forceinline__ void warp_maxima(float (&v)[kB]) {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  for (int o = 16; o >= 1; o >>= 1)
+#pragma unroll
+    for (int b = 0; b < kB; ++b) v[b] = fmaxf(v[b], __shfl_xor_sync(0xffffffffu, v[b], o));
 }
 
 struct BalArgs {
@@ -79,51 +117,84 @@ __device__ __forceinline__ void bal_bounds(const BalArgs& a, int s, int64_t* lo,
   *hi = h < *lo ? *lo : (h > a.T ? a.T : h);
 }
 
-// First sequence that ends after token t (S if none).
+// First sequence that ends after token t (S if none): the number of those that
+// do not, counted by the whole CTA (one load deep, where a search is five or more).
 __device__ __forceinline__ int bal_first(const BalArgs& a, int64_t t) {
   if (!a.off) return 0;
-  int lo = 0, hi = a.S;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.off[mid + 1] > t)
-      hi = mid;
-    else
-      lo = mid + 1;
+  int n = 0;
+  for (int s0 = 0; s0 < a.S; s0 += kBalThreads) {
+    const int s = s0 + threadIdx.x;
+    const int got = __syncthreads_count(s < a.S && a.off[s + 1] <= t);
+    n += got;
+    if (got < kBalThreads) break;
   }
-  return lo;
+  return n;
 }
 
-// The warp's row: scores x[j] -> a_j (columns lane + 32 j), returns 1 / sum (0
-// for a row whose scores sum to zero).
-template <int kJ>
-__device__ __forceinline__ float bal_scores(float (&x)[kJ], int lane, int E, int softmax) {
-  float z = 0.f;
-  if (softmax) {
-    float m = -INFINITY;
+// The logits of rows t, t + kBalWarps, ... (nb of them, at most kB) -> scores
+// a_j (0 in columns that are not there); rz: 1 / their sum, 0 where the scores
+// sum to zero.
+template <int kDt, int kV, int kJ, int kB>
+__device__ __forceinline__ void bal_scores(const BalArgs& a, int64_t t, int nb, int lane, float (&x)[kB][kJ * kV],
+                                           float (&rz)[kB]) {
+  constexpr int kSize = kDt == 2 ? 4 : 2;
 #pragma unroll
-    for (int j = 0; j < kJ; ++j)
-      if (lane + 32 * j < E) m = fmaxf(m, x[j]);
-    m = warp_max(m);
-    // a row of -inf: exp(-inf - 0) = 0 everywhere (a NaN row keeps its NaN)
-    if (m == -INFINITY) m = 0.f;
+  for (int b = 0; b < kB; ++b) {
+    if (b >= nb) break;
+    const uint8_t* row = static_cast<const uint8_t*>(a.logits) + (t + b * kBalWarps) * a.ld * kSize;
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      x[j] = lane + 32 * j < E ? expf(x[j] - m) : 0.f;
-      z += x[j];
-    }
-  } else {
+      const int c = (j * 32 + lane) * kV;
+      if (c < a.E) {
+        bal_load<kDt, kV>(row, c, &x[b][j * kV]);
+      } else {
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) {
-      x[j] = lane + 32 * j < E ? 1.0f / (1.0f + expf(-x[j])) : 0.f;
-      z += x[j];
+        for (int v = 0; v < kV; ++v) x[b][j * kV + v] = -INFINITY;  // scores 0
+      }
     }
   }
-  z = warp_sum(z);
-  return z == 0.f ? 0.f : 1.0f / z;
+  float m[kB];
+  if (a.softmax) {
+#pragma unroll
+    for (int b = 0; b < kB; ++b) {
+      m[b] = -INFINITY;
+      if (b >= nb) continue;
+#pragma unroll
+      for (int i = 0; i < kJ * kV; ++i) m[b] = fmaxf(m[b], x[b][i]);
+    }
+    warp_maxima(m);
+  }
+#pragma unroll
+  for (int b = 0; b < kB; ++b) {
+    rz[b] = 0.f;
+    if (b >= nb) continue;
+    if (a.softmax) {
+      // a row of -inf: exp(-inf - 0) = 0 everywhere (a NaN row keeps its NaN)
+      const float top = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int i = 0; i < kJ * kV; ++i) x[b][i] = expf(x[b][i] - top);
+    } else {
+      // the quotient within 2 steps of float32 (0 below 2^-126), a third of a division's operations
+#pragma unroll
+      for (int i = 0; i < kJ * kV; ++i) x[b][i] = __fdividef(1.0f, 1.0f + expf(-x[b][i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kJ * kV; ++i) rz[b] += x[b][i];
+  }
+  warp_sums(rz);
+#pragma unroll
+  for (int b = 0; b < kB; ++b) rz[b] = rz[b] == 0.f ? 0.f : 1.0f / rz[b];
+}
+
+// Rows of a warp's next batch: t, t + kBalWarps, ... below hi.
+template <int kB>
+__device__ __forceinline__ int bal_rows(int64_t t, int64_t hi) {
+  const int64_t n = (hi - t + kBalWarps - 1) / kBalWarps;
+  return n < kB ? static_cast<int>(n) : kB;
 }
 
 // Slot layout: psum float [slots][E], pcnt int32 [slots][E].
-template <int kDt, int kJ>
+template <int kDt, int kV, int kJ>
 __global__ void __launch_bounds__(kBalThreads)
     balance_partial_kernel(BalArgs a, float* __restrict__ psum, int32_t* __restrict__ pcnt) {
   extern __shared__ float sm[];  // [kBalWarps][E] column sums, then [E] counts
@@ -133,7 +204,6 @@ __global__ void __launch_bounds__(kBalThreads)
   griddep_launch_dependents();
   const int64_t t0 = blockIdx.x * static_cast<int64_t>(a.run);
   const int64_t t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
-  constexpr int kSize = kDt == 2 ? 4 : 2;
   for (int s = bal_first(a, t0); s < a.S; ++s) {
     int64_t lo, hi;
     bal_bounds(a, s, &lo, &hi);
@@ -142,28 +212,34 @@ __global__ void __launch_bounds__(kBalThreads)
     hi = hi < t1 ? hi : t1;
     if (lo >= hi) continue;
     for (int c = tid; c < a.E; c += kBalThreads) cnt[c] = 0;
-    float acc[kJ];
-#pragma unroll
-    for (int j = 0; j < kJ; ++j) acc[j] = 0.f;
-    for (int64_t t = lo + warp; t < hi; t += kBalWarps) {
-      const uint8_t* row = static_cast<const uint8_t*>(a.logits) + t * a.ld * kSize;
-      float x[kJ];
-#pragma unroll
-      for (int j = 0; j < kJ; ++j)
-        if (lane + 32 * j < a.E) x[j] = bal_load<kDt>(row, lane + 32 * j);
-      const float rz = bal_scores<kJ>(x, lane, a.E, a.softmax);
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) acc[j] = fmaf(x[j], rz, acc[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < kJ; ++j)
-      if (lane + 32 * j < a.E) sm[warp * a.E + lane + 32 * j] = acc[j];
     __syncthreads();
     const int64_t n = (hi - lo) * a.K;
     for (int64_t i = tid; i < n; i += kBalThreads) {
       const int32_t id = a.ids[lo * a.K + i];
       if (static_cast<uint32_t>(id) < static_cast<uint32_t>(a.E)) atomicAdd(&cnt[id], 1);
     }
+    float acc[kJ * kV];
+#pragma unroll
+    for (int i = 0; i < kJ * kV; ++i) acc[i] = 0.f;
+    constexpr int kB = bal_batch(kJ * kV);
+    for (int64_t t = lo + warp; t < hi; t += kB * kBalWarps) {
+      float x[kB][kJ * kV], rz[kB];
+      const int nb = bal_rows<kB>(t, hi);
+      bal_scores<kDt, kV, kJ, kB>(a, t, nb, lane, x, rz);
+#pragma unroll
+      for (int b = 0; b < kB; ++b) {
+        if (b >= nb) break;
+#pragma unroll
+        for (int i = 0; i < kJ * kV; ++i) acc[i] = fmaf(x[b][i], rz[b], acc[i]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        const int c = (j * 32 + lane) * kV + v;
+        if (c < a.E) sm[warp * a.E + c] = acc[j * kV + v];
+      }
     __syncthreads();
     const int64_t slot = blockIdx.x + static_cast<int64_t>(s);
     for (int c = tid; c < a.E; c += kBalThreads) {
@@ -177,16 +253,18 @@ __global__ void __launch_bounds__(kBalThreads)
   }
 }
 
-constexpr int kBalFinThreads = 512;
+constexpr int kBalFinThreads = 1024;
 
-// One CTA a sequence: thread groups of 32 columns x 16 slot lanes.
+// One CTA a sequence: 128 columns at a time x 8 threads, which take every
+// eighth slot each, sixteen loads in flight.
 __global__ void __launch_bounds__(kBalFinThreads)
     balance_final_kernel(BalArgs a, const float* __restrict__ psum, const int32_t* __restrict__ pcnt,
                          float* __restrict__ loss, int32_t* __restrict__ counts) {
-  constexpr int kLanes = kBalFinThreads / 32;
-  __shared__ double ssum[kLanes][32];
-  __shared__ int32_t scnt[kLanes][32];
-  const int tid = threadIdx.x, lane = tid & 31, part = tid >> 5;
+  constexpr int kCols = 128, kParts = kBalFinThreads / kCols;
+  __shared__ double ssum[kParts][kCols];
+  __shared__ int32_t scnt[kParts][kCols];
+  __shared__ double wsum[kCols / 32];
+  const int tid = threadIdx.x, col = tid % kCols, part = tid / kCols;
   const int s = blockIdx.x;
   griddep_wait();
   griddep_launch_dependents();
@@ -194,27 +272,27 @@ __global__ void __launch_bounds__(kBalFinThreads)
   bal_bounds(a, s, &lo, &hi);
   const int64_t c0 = lo / a.run + s, c1 = lo < hi ? (hi - 1) / a.run + s + 1 : c0;
   double total = 0.0;
-  for (int e0 = 0; e0 < a.E; e0 += 32) {
-    const int e = e0 + lane;
+  for (int e0 = 0; e0 < a.E; e0 += kCols) {
+    const int e = e0 + col;
     double p = 0.0;
     int32_t n = 0;
     if (e < a.E) {
-#pragma unroll 4
-      for (int64_t k = c0 + part; k < c1; k += kLanes) {
+#pragma unroll 8
+      for (int64_t k = c0 + part; k < c1; k += kParts) {
         p += psum[k * a.E + e];
         n += pcnt[k * a.E + e];
       }
     }
-    ssum[part][lane] = p;
-    scnt[part][lane] = n;
+    ssum[part][col] = p;
+    scnt[part][col] = n;
     __syncthreads();
     if (part == 0 && e < a.E) {
       p = 0.0;
       n = 0;
 #pragma unroll
-      for (int w = 0; w < kLanes; ++w) {
-        p += ssum[w][lane];
-        n += scnt[w][lane];
+      for (int w = 0; w < kParts; ++w) {
+        p += ssum[w][col];
+        n += scnt[w][col];
       }
       counts[static_cast<int64_t>(s) * a.E + e] = n;
       total += p * n;
@@ -224,16 +302,21 @@ __global__ void __launch_bounds__(kBalFinThreads)
   if (part == 0) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) {
-      const double len = static_cast<double>(hi - lo);
-      loss[s] = hi > lo ? static_cast<float>(a.coeff * total * a.E / (a.K * len * len)) : 0.f;
-    }
+    if ((col & 31) == 0) wsum[col / 32] = total;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kCols / 32; ++w) total += wsum[w];
+    const double len = static_cast<double>(hi - lo);
+    loss[s] = hi > lo ? static_cast<float>(a.coeff * total * a.E / (a.K * len * len)) : 0.f;
   }
 }
 
-// Gradient of sum_s grad_loss[s] * loss[s]: one warp a token, f of the
-// token's sequence in registers.
-template <int kDt, int kJ>
+// Gradient of sum_s grad_loss[s] * loss[s]: a warp takes some tokens at a
+// time, f of their sequence in registers.
+template <int kDt, int kV, int kJ>
 __global__ void __launch_bounds__(kBalThreads)
     balance_backward_kernel(BalArgs a, const int32_t* __restrict__ counts, const float* __restrict__ grad_loss,
                             void* __restrict__ grad) {
@@ -245,9 +328,10 @@ __global__ void __launch_bounds__(kBalThreads)
   constexpr int kSize = kDt == 2 ? 4 : 2;
   int64_t done = t0;  // tokens before this one have their gradient
   auto zero = [&](int64_t lo, int64_t hi) {
+    const float z[1] = {0.f};
     for (int64_t t = lo + warp; t < hi; t += kBalWarps) {
       uint8_t* row = static_cast<uint8_t*>(grad) + t * a.E * kSize;
-      for (int c = lane; c < a.E; c += 32) bal_store<kDt>(row, c, 0.f);
+      for (int c = lane; c < a.E; c += 32) bal_store<kDt, 1>(row, c, z);
     }
   };
   for (int s = bal_first(a, t0); s < a.S; ++s) {
@@ -261,27 +345,45 @@ __global__ void __launch_bounds__(kBalThreads)
     zero(done, lo);
     const float unit = static_cast<float>(a.E) / (static_cast<float>(a.K) * len);
     const float g = grad_loss[s] * a.coeff / len;
-    float f[kJ];
+    float f[kJ * kV];
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
-      f[j] = lane + 32 * j < a.E ? unit * static_cast<float>(counts[static_cast<int64_t>(s) * a.E + lane + 32 * j]) : 0.f;
-    for (int64_t t = lo + warp; t < hi; t += kBalWarps) {
-      const uint8_t* row = static_cast<const uint8_t*>(a.logits) + t * a.ld * kSize;
-      uint8_t* out = static_cast<uint8_t*>(grad) + t * a.E * kSize;
-      float x[kJ];
 #pragma unroll
-      for (int j = 0; j < kJ; ++j)
-        if (lane + 32 * j < a.E) x[j] = bal_load<kDt>(row, lane + 32 * j);
-      const float rz = bal_scores<kJ>(x, lane, a.E, a.softmax);
-      float dot = 0.f;
+      for (int v = 0; v < kV; ++v) {
+        const int c = (j * 32 + lane) * kV + v;
+        f[j * kV + v] = c < a.E ? unit * static_cast<float>(counts[static_cast<int64_t>(s) * a.E + c]) : 0.f;
+      }
+    constexpr int kB = bal_batch(kJ * kV);
+    for (int64_t t = lo + warp; t < hi; t += kB * kBalWarps) {
+      float x[kB][kJ * kV], rz[kB], dot[kB];
+      const int nb = bal_rows<kB>(t, hi);
+      bal_scores<kDt, kV, kJ, kB>(a, t, nb, lane, x, rz);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) dot = fmaf(f[j], x[j], dot);
-      dot = warp_sum(dot) * rz;
+      for (int b = 0; b < kB; ++b) {
+        dot[b] = 0.f;
+        if (b >= nb) continue;
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        float d = g * (x[j] * rz) * (f[j] - dot);
-        if (!a.softmax) d *= 1.0f - x[j];
-        if (lane + 32 * j < a.E) bal_store<kDt>(out, lane + 32 * j, d);
+        for (int i = 0; i < kJ * kV; ++i) dot[b] = fmaf(f[i], x[b][i], dot[b]);
+      }
+      warp_sums(dot);
+#pragma unroll
+      for (int b = 0; b < kB; ++b) {
+        if (b >= nb) break;
+        const int64_t r = t + b * kBalWarps;
+        const float mean = dot[b] * rz[b];
+        uint8_t* row = static_cast<uint8_t*>(grad) + r * a.E * kSize;
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          const int c = (j * 32 + lane) * kV;
+          float d[kV];
+#pragma unroll
+          for (int v = 0; v < kV; ++v) {
+            const float y = x[b][j * kV + v];
+            d[v] = g * (y * rz[b]) * (f[j * kV + v] - mean);
+            if (!a.softmax) d[v] *= 1.0f - y;
+          }
+          if (c < a.E) bal_store<kDt, kV>(row, c, d);
+        }
       }
     }
     done = hi;
@@ -289,15 +391,25 @@ __global__ void __launch_bounds__(kBalThreads)
   zero(done, t1);
 }
 
-// Tokens of a CTA: two CTAs' worth on every SM before runs grow past 16 tokens.
+// Tokens of a CTA: one CTA on every SM before runs grow past a batch of every warp.
 int bal_run(int64_t T) {
-  const int64_t per = (T + 2 * kSMs - 1) / (2 * kSMs);
+  const int64_t per = (T + kSMs - 1) / kSMs;
   return static_cast<int>(per < 16 ? 16 : per);
 }
 
-#define BAL_J(KERNEL, D)                                             \
-  (E <= 32 ? KERNEL<D, 1> : E <= 64 ? KERNEL<D, 2> : E <= 128 ? KERNEL<D, 4> \
-   : E <= 256 ? KERNEL<D, 8> : E <= 512 ? KERNEL<D, 16> : KERNEL<D, 32>)
+// Vector columns where every row of 4 is aligned.
+bool bal_vector(const BalanceCall& c, const void* grad) {
+  const int64_t size = c.dt == 2 ? 4 : 2;
+  return c.E % 4 == 0 && c.ld % 4 == 0 && reinterpret_cast<uintptr_t>(c.logits) % (4 * size) == 0 &&
+         reinterpret_cast<uintptr_t>(grad) % (4 * size) == 0;
+}
+
+#define BAL_DT(KERNEL, V, J) (dt == 0 ? KERNEL<0, V, J> : dt == 1 ? KERNEL<1, V, J> : KERNEL<2, V, J>)
+#define BAL_PICK(KERNEL)                                                                                      \
+  (vec ? (E <= 128 ? BAL_DT(KERNEL, 4, 1) : E <= 256 ? BAL_DT(KERNEL, 4, 2)                                   \
+                   : E <= 512 ? BAL_DT(KERNEL, 4, 4) : BAL_DT(KERNEL, 4, 8))                                  \
+       : (E <= 32 ? BAL_DT(KERNEL, 1, 1) : E <= 128 ? BAL_DT(KERNEL, 1, 4)                                    \
+                  : E <= 512 ? BAL_DT(KERNEL, 1, 16) : BAL_DT(KERNEL, 1, 32)))
 
 BalArgs bal_args(const BalanceCall& c) {
   BalArgs a{};
@@ -315,7 +427,7 @@ BalArgs bal_args(const BalanceCall& c) {
   return a;
 }
 
-uint32_t bal_grid(const BalArgs& a) { return static_cast<uint32_t>((a.T + a.run - 1) / a.run); }
+dim3 bal_grid(const BalArgs& a) { return dim3(static_cast<uint32_t>((a.T + a.run - 1) / a.run)); }
 
 }  // namespace
 
@@ -326,14 +438,18 @@ int64_t balance_slots(int64_t T, int64_t S) {
 
 cudaError_t launch_balance(const BalanceCall& c, void* work, float* loss, int32_t* counts, cudaStream_t s) {
   const BalArgs a = bal_args(c);
-  const int E = c.E;
+  const int E = c.E, dt = c.dt;
+  const bool vec = bal_vector(c, nullptr);
   float* psum = static_cast<float*>(work);
   int32_t* pcnt = reinterpret_cast<int32_t*>(psum + balance_slots(c.T, c.S) * E);
   if (a.T > 0) {
-    auto k = c.dt == 0 ? BAL_J(balance_partial_kernel, 0) : c.dt == 1 ? BAL_J(balance_partial_kernel, 1)
-                                                                       : BAL_J(balance_partial_kernel, 2);
-    const size_t smem = static_cast<size_t>(kBalWarps + 1) * E * 4;  // 36 KB at E = 1024
-    const cudaError_t e = launch_k(k, dim3(bal_grid(a)), dim3(kBalThreads), smem, s, true, a, psum, pcnt);
+    auto k = BAL_PICK(balance_partial_kernel);
+    const size_t smem = static_cast<size_t>(kBalWarps + 1) * E * 4;  // 68 KB at E = 1024
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (e != cudaSuccess) return e;
+    }
+    const cudaError_t e = launch_k(k, bal_grid(a), dim3(kBalThreads), smem, s, true, a, psum, pcnt);
     if (e != cudaSuccess) return e;
   }
   return launch_k(balance_final_kernel, dim3(c.S), dim3(kBalFinThreads), 0, s, true, a,
@@ -344,10 +460,10 @@ cudaError_t launch_balance_backward(const BalanceCall& c, const int32_t* counts,
                                     cudaStream_t s) {
   if (c.T == 0) return cudaSuccess;
   const BalArgs a = bal_args(c);
-  const int E = c.E;
-  auto k = c.dt == 0 ? BAL_J(balance_backward_kernel, 0) : c.dt == 1 ? BAL_J(balance_backward_kernel, 1)
-                                                                      : BAL_J(balance_backward_kernel, 2);
-  return launch_k(k, dim3(bal_grid(a)), dim3(kBalThreads), 0, s, true, a, counts, grad_loss, grad);
+  const int E = c.E, dt = c.dt;
+  const bool vec = bal_vector(c, grad);
+  auto k = BAL_PICK(balance_backward_kernel);
+  return launch_k(k, bal_grid(a), dim3(kBalThreads), 0, s, true, a, counts, grad_loss, grad);
 }
 
 }  // namespace moe
