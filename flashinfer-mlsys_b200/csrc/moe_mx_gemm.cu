@@ -80,6 +80,7 @@ struct MxGemmArgs {
   int nsc;             // scales of a row
   int nk;              // stages of K
   int tn;              // tokens of a tile (multiple of 16, <= kNT)
+  int box;             // token rows of one copy
   int split;           // CTAs of a cluster, each with its share of K
 };
 
@@ -413,26 +414,30 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     // ======================= TMA producer =======================
     if (lane == 0) {
       uint32_t it = 0;
-      const int rows_a = kPair ? p.tn / 2 : p.tn;  // token rows of this CTA's box
       for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
         const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
-        // the second CTA of a pair holds the second half of the columns that are issued
-        const int row_a = x.row0 + (kPair ? rank * ((x.cnt + 15) / 16 * 8) : 0);
+        // token rows of this CTA: the columns that are issued, of which the
+        // second CTA of a pair holds the second half
+        const int rows_a = (x.cnt + 15) / 16 * (kPair ? 8 : 16);
+        const int row_a = x.row0 + (kPair ? rank * rows_a : 0);
+        const int boxes = (rows_a + p.box - 1) / p.box;
+        const uint32_t bytes = Cfg::kTileBytes + boxes * p.box * kMxStageK;
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % kS;
           if (!mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs)) { mx_abort(ctl); break; }
           uint8_t* st = tiles + s * Cfg::kStageBytes;
-          const uint32_t bytes = Cfg::kTileBytes + rows_a * kMxStageK;
           if constexpr (kPair) {
             // both CTAs' copies count on the first CTA's barrier
             const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
             if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * bytes);
             tma_load_3d_pair(st, &map_w, k * kMxStageK, x.n0 + my_n, x.e, bar);
-            tma_load_3d_pair(st + Cfg::kTileBytes, &map_a, k * kMxStageK, row_a, 0, bar);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d_pair(st + Cfg::kTileBytes + b * p.box * kMxStageK, &map_a, k * kMxStageK, row_a + b * p.box, 0, bar);
           } else {
             mbar_arrive_expect_tx(&ctl->full[s], bytes);
             tma_load_3d(st, &map_w, k * kMxStageK, x.n0, x.e, &ctl->full[s]);
-            tma_load_3d(st + Cfg::kTileBytes, &map_a, k * kMxStageK, row_a, 0, &ctl->full[s]);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d(st + Cfg::kTileBytes + b * p.box * kMxStageK, &map_a, k * kMxStageK, row_a + b * p.box, 0, &ctl->full[s]);
           }
         }
       }
@@ -736,16 +741,16 @@ cudaError_t mx_gemm_launch_nt(const MxPlan& pl, const CUtensorMap& mw, const CUt
 // One run of rows: the tile width that gives the least (waves of CTAs) x
 // (rows loaded per stage). Several runs, whose lengths only the device knows:
 // by their mean length.
-#ifndef MX_PAIR_ABOVE
-#define MX_PAIR_ABOVE 128
-#endif
+// Token rows of a copy where the runs' lengths are known to the device only: a
+// short tile then loads little more than it has.
+constexpr int kMxRunBox = 64;
 MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs) {
   const int sms = device_sm_count();
   const int64_t ntn = (N + kMxTileN - 1) / kMxTileN;
   MxPlan pl{};
   if (runs) {
     const int64_t mean = (rows + experts - 1) / experts;
-    pl.tn = mean <= 8 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 160 ? 128 : 256;
+    pl.tn = mean <= 8 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : 256;
   } else if (rows <= 64) {
     pl.tn = static_cast<int>((rows + 15) / 16 * 16);
   } else {
@@ -760,13 +765,13 @@ MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs) {
     }
   }
   // wide tiles: a pair of CTAs, each with half of the tokens in shared memory
-  pl.pair = pl.tn > MX_PAIR_ABOVE;
+  pl.pair = pl.tn > 128;
   if (pl.pair) {
     const int64_t tiles = (N + 2 * kMxTileN - 1) / (2 * kMxTileN) * (rows / pl.tn + (runs ? (experts < rows ? experts : rows) : 1));
     pl.nt = 256;
     pl.split = 1;
     pl.grid = static_cast<int>(2 * (tiles < sms / 2 ? tiles : sms / 2));
-    pl.box_rows = pl.tn / 2;
+    pl.box_rows = runs ? kMxRunBox : pl.tn / 2;
     return pl;
   }
   pl.box_rows = pl.tn;
@@ -798,6 +803,7 @@ cudaError_t launch_mx_gemm(const CUtensorMap& map_w, const CUtensorMap& map_a, c
   p.nsc = static_cast<int>(c.K / mx_block(c.fmt));
   p.nk = mx_gemm_stages(c.K, c.fmt);
   p.tn = pl.tn;
+  p.box = pl.box_rows;
   p.split = pl.split;
   switch (c.fmt) {
     case kFmtNvfp4: return mx_gemm_launch_nt<kFmtNvfp4>(pl, map_w, map_a, p, s);
