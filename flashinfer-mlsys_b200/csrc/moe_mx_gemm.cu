@@ -276,36 +276,61 @@ __device__ __forceinline__ void mx_out_store(const MxGemmArgs& p, int64_t row, i
     static_cast<float*>(p.out)[i] = v;
 }
 
-// The scale words of one row and stage: `left` scales remain in the row from
-// `s` on (none: zeros). kVec: rows are whole stages, aligned to one; otherwise
-// words where every row is, or bytes.
-template <int kW, bool kVec>
-__device__ __forceinline__ void mx_sf_load(const uint8_t* s, int left, bool words, uint32_t (&w)[kW]) {
+// The scale words of one row and stage, kA bytes a load (rows and base are
+// aligned to kA); `left` scales remain in the row, none or less: zeros. Rows
+// that are whole stages, the usual ones, take one load, skipped where there is
+// nothing. Of several loads, those past the end go to `safe`, and
+// `word` below drops what they bring: a branch around each took some hundred cycles.
+template <int kW, int kA>
+__device__ __forceinline__ void mx_sf_aligned(const uint8_t* s, int left, const uint8_t* safe, uint32_t* w) {
+  constexpr bool kWhole = kA == 4 * kW;
+  if (kWhole) {
 #pragma unroll
-  for (int i = 0; i < kW; ++i) w[i] = 0;
-  if constexpr (kVec) {
-    if (left > 0) {
-      if constexpr (kW == 4) {
-        uint4 v;  // volatile: stays before the wait for the slot
-        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(s));
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-      } else if constexpr (kW == 2) {
-        uint2 v;
-        asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(s));
-        w[0] = v.x, w[1] = v.y;
-      } else {
-        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[0]) : "l"(s));
+    for (int i = 0; i < kW; ++i) w[i] = 0;
+    if (left <= 0) return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * kW; i += kA) {
+    const uint8_t* q = kWhole || i < left ? s + i : safe;
+    uint32_t* d = w + i / 4;
+    // volatile: the loads stay before the wait for the slot
+    if constexpr (kA == 16)
+      asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "l"(q));
+    else if constexpr (kA == 8)
+      asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "l"(q));
+    else
+      asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(d[0]) : "l"(q));
+  }
+}
+
+// Rows of any length: the kW + 1 aligned words around the bytes, shifted into
+// place by mx_sf_shift. `inside`: all of them lie in the tensor; otherwise the
+// words are put together from those bytes that lie in [begin, end).
+template <int kW>
+__device__ __forceinline__ void mx_sf_around(const uint8_t* s, int left, bool inside, const uint8_t* begin,
+                                             const uint8_t* end, uint32_t* v) {
+  if (inside) {
+    const uint8_t* a = left > 0 ? s - (reinterpret_cast<uintptr_t>(s) & 3u) : begin;
+#pragma unroll
+    for (int i = 0; i <= kW; ++i) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v[i]) : "l"(a + 4 * i));
+  } else {
+    const uint8_t* a = s - (reinterpret_cast<uintptr_t>(s) & 3u);
+#pragma unroll
+    for (int i = 0; i <= kW; ++i) {
+      v[i] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint8_t* q = a + 4 * i + b;
+        if (left > 0 && q >= begin && q < end) v[i] |= static_cast<uint32_t>(__ldg(q)) << (8 * b);
       }
     }
-  } else if (words) {
-#pragma unroll
-    for (int i = 0; i < kW; ++i)
-      if (4 * i < left) w[i] = __ldg(reinterpret_cast<const uint32_t*>(s) + i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4 * kW; ++i)
-      if (i < left) w[i / 4] |= static_cast<uint32_t>(__ldg(s + i)) << (8 * (i % 4));
   }
+}
+// Word i of a row's stage from the words around it; scales past the row's end are 0.
+__device__ __forceinline__ uint32_t mx_sf_shift(const uint32_t* v, int i, int off, int left) {
+  const uint32_t w = __funnelshift_r(v[i], v[i + 1], 8 * off);
+  const int keep = left - 4 * i;  // bytes of this word that belong to the row
+  return keep >= 4 ? w : (keep > 0 ? w & (0xFFFFFFFFu >> (8 * (4 - keep))) : 0u);
 }
 
 // A bounded wait gives up for the whole warp or for none of it.
@@ -370,22 +395,32 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   }
   griddep_wait();
   griddep_launch_dependents();
-  // runs and their token tiles: one warp, 32 experts at a time
-  if (warp == 2) {
-    int base = 0;
+  // Runs and their token tiles: one warp, 32 experts at a time. Bounds are kept
+  // inside [0, R] and made not to decrease, so that the runs are disjoint
+  // whatever the offsets hold.
+  if (!p.off) {
+    if (tid == 64) {
+      ctl->start[0] = 0;
+      ctl->count[0] = p.R;
+      ctl->prefix[0] = 0;
+      ctl->prefix[1] = (p.R + p.tn - 1) / p.tn;
+    }
+  } else if (warp == 2) {
+    int tiles = 0, from = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int e = e0 + lane;
-      int lo = 0, hi = 0;
+      int lo = from, hi = from;
       if (e < p.E) {
-        if (p.off) {  // kept inside [0, R] whatever the offsets hold
-          lo = min(max(__ldg(p.off + e), 0), p.R);
-          hi = min(max(__ldg(p.off + e + 1), lo), p.R);
-        } else {
-          hi = p.R;
-        }
-        ctl->start[e] = lo;
-        ctl->count[e] = hi - lo;
+        lo = min(max(__ldg(p.off + e), from), p.R);
+        hi = min(max(__ldg(p.off + e + 1), lo), p.R);
       }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {  // running maximum of the ends
+        const int v = __shfl_up_sync(0xffffffffu, hi, o);
+        if (lane >= o) hi = max(hi, v);
+      }
+      const int before = __shfl_up_sync(0xffffffffu, hi, 1);
+      if (lane > 0) lo = max(lo, before);
       const int t = (hi - lo + p.tn - 1) / p.tn;
       int inc = t;
 #pragma unroll
@@ -393,10 +428,15 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         const int v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
       }
-      if (e < p.E) ctl->prefix[e] = base + inc - t;
-      base += __shfl_sync(0xffffffffu, inc, 31);
+      if (e < p.E) {
+        ctl->start[e] = lo;
+        ctl->count[e] = hi - lo;
+        ctl->prefix[e] = tiles + inc - t;
+      }
+      tiles += __shfl_sync(0xffffffffu, inc, 31);
+      from = __shfl_sync(0xffffffffu, hi, 31);
     }
-    if (lane == 0) ctl->prefix[p.E] = base;
+    if (lane == 0) ctl->prefix[p.E] = tiles;
   }
   tc_fence_before();
   if (clustered)
@@ -543,28 +583,54 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     const int r0 = (warp - kMxSfWarp0) * 8 + (lane & 7), j = lane >> 3;
     const uint64_t low =
         reinterpret_cast<uint64_t>(p.sw) | reinterpret_cast<uint64_t>(p.sa) | static_cast<uint64_t>(p.nsc);
-    const bool words = (low & 3) == 0;
-    // one loop for each kind of row, so that the usual one has no branches
-    // among its loads: with them it waited for every load where it stood
-    const auto loop = [&](auto vec) {
-    constexpr bool kVec = decltype(vec)::value;
-    // the words of stages k .. k + 3 of unit x
-    const auto load = [&](const MxUnit& x, int k, uint32_t (&w)[1 + Cfg::kChunks][4][kW]) {
+    const uint8_t* end_w = p.sw + static_cast<int64_t>(p.E) * p.N * p.nsc;
+    const uint8_t* end_a = p.sa + static_cast<int64_t>(p.R) * p.nsc;
+    // one loop for each kind of row, so that there are no branches among the loads
+    const auto loop = [&](auto align) {
+    constexpr int kA = decltype(align)::value;  // bytes of a load; 1: words around the bytes
+    constexpr int kR = kA > 1 ? kW : kW + 1;    // words held of a row and stage
+    const int64_t ld = p.nsc;
+    // the words of stages k .. k + 3 of unit x: 128-row group g = 0 is the
+    // weights', the others the tokens'
+    const auto load = [&](const MxUnit& x, int k, uint32_t (&w)[1 + Cfg::kChunks][4][kR]) {
       const int n0 = x.n0 + my_n;
-      const uint8_t* bw = p.sw + (static_cast<int64_t>(x.e) * p.N + n0) * p.nsc;
-      const uint8_t* ba = p.sa + static_cast<int64_t>(x.row0) * p.nsc;
-      const int at = (k + j) * 4 * kW, left = k + j < k1 ? p.nsc - at : 0;
+      const int at = (k + j) * 4 * kW;
+      const int left = k + j < k1 ? p.nsc - at : 0;
+      const uint8_t* base[2] = {p.sw + (static_cast<int64_t>(x.e) * p.N + n0) * ld, p.sa + x.row0 * ld};
+      bool inside = true;
+      if constexpr (kA == 1) {
+        // the four stages' words of the last row of either side
+        const int64_t last = static_cast<int64_t>(k + 4) * 4 * kW + 4;
+        inside = (reinterpret_cast<uint64_t>(p.sw) & 3) == 0 && (reinterpret_cast<uint64_t>(p.sa) & 3) == 0 &&
+                 base[0] + (min(kMxTileN, p.N - n0) - 1) * ld + last <= end_w && base[1] + (x.cnt - 1) * ld + last <= end_a;
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int r = r0 + 32 * q;
-        mx_sf_load<kW, kVec>(bw + static_cast<int64_t>(r) * p.nsc + at, r < p.N - n0 ? left : 0, words, w[0][q]);
 #pragma unroll
-        for (int c = 0; c < Cfg::kChunks; ++c)
-          mx_sf_load<kW, kVec>(ba + static_cast<int64_t>(c * 128 + r) * p.nsc + at, c * 128 + r < x.cnt ? left : 0, words,
-                               w[1 + c][q]);
+        for (int g = 0; g <= Cfg::kChunks; ++g) {
+          const int r = r0 + 32 * q + (g > 1 ? 128 : 0);
+          const int mine = r < (g == 0 ? p.N - n0 : x.cnt) ? left : 0;
+          const uint8_t* s = base[g > 0] + r * ld + at;
+          if constexpr (kA > 1)
+            mx_sf_aligned<kW, kA>(s, mine, g == 0 ? p.sw : p.sa, w[g][q]);
+          else
+            mx_sf_around<kW>(s, mine, inside, g == 0 ? p.sw : p.sa, g == 0 ? end_w : end_a, w[g][q]);
+        }
       }
     };
-    uint32_t w[1 + Cfg::kChunks][4][kW];
+    // word i of row q of group g, of the stage that this lane loaded
+    const auto word = [&](const MxUnit& x, int k, const uint32_t (&w)[1 + Cfg::kChunks][4][kR], int g, int q, int i) {
+      if constexpr (kA == 4 * kW) return w[g][q][i];
+      const int r = r0 + 32 * q + (g > 1 ? 128 : 0), at = (k + j) * 4 * kW;
+      const int left = k + j < k1 && r < (g == 0 ? p.N - x.n0 - my_n : x.cnt) ? p.nsc - at : 0;
+      if constexpr (kA > 1) {
+        return 4 * i < left ? w[g][q][i] : 0u;
+      } else {
+        const uint8_t* b = g == 0 ? p.sw + (static_cast<int64_t>(x.e) * p.N + x.n0 + my_n) * ld : p.sa + x.row0 * ld;
+        return mx_sf_shift(w[g][q], i, static_cast<int>((reinterpret_cast<uint64_t>(b) + r * ld + at) & 3u), left);
+      }
+    };
+    uint32_t w[1 + Cfg::kChunks][4][kR];
     uint32_t grp = 0;
     for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
       const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
@@ -577,11 +643,10 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
 #pragma unroll
         for (int i = 0; i < kW; ++i) {
-          *reinterpret_cast<uint4*>(sf + i * 512) = make_uint4(w[0][0][i], w[0][1][i], w[0][2][i], w[0][3][i]);
 #pragma unroll
-          for (int c = 0; c < Cfg::kChunks; ++c)
-            *reinterpret_cast<uint4*>(sf + kW * 512 + (i * Cfg::kChunks + c) * 512) =
-                make_uint4(w[1 + c][0][i], w[1 + c][1][i], w[1 + c][2][i], w[1 + c][3][i]);
+          for (int g = 0; g <= Cfg::kChunks; ++g)
+            *reinterpret_cast<uint4*>(sf + (g == 0 ? i : kW + i * Cfg::kChunks + g - 1) * 512) =
+                make_uint4(word(x, k, w, g, 0, i), word(x, k, w, g, 1, i), word(x, k, w, g, 2, i), word(x, k, w, g, 3, i));
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -590,10 +655,14 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (!ok) { mx_abort(ctl); break; }
     }
     };
-    if ((low & (4 * kW - 1)) == 0)
-      loop(std::true_type{});
+    if (kW == 4 && (low & 15) == 0)
+      loop(std::integral_constant<int, kW == 4 ? 16 : 4>{});
+    else if (kW >= 2 && (low & 7) == 0)
+      loop(std::integral_constant<int, kW >= 2 ? 8 : 4>{});
+    else if ((low & 3) == 0)
+      loop(std::integral_constant<int, 4>{});
     else
-      loop(std::false_type{});
+      loop(std::integral_constant<int, 1>{});
   } else {
     // ======================= epilogue (8 warps) =======================
     const int q = warp & 3, half = (warp - kMxEpiWarp0) >> 2;

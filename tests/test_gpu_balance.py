@@ -155,6 +155,35 @@ def test_empty_repeat_graph_and_backward_twice(gpu_available):
     assert torch.equal(cg.cpu().long(), n)
 
 
+def test_second_derivative_is_refused(gpu_available):
+    x, ids, off, _ = _inputs(8, 16, 2, 1, torch.float32, 9)
+    xd = x.to(DEV).requires_grad_(True)
+    loss, _ = pkg().balance_loss(xd, ids.to(DEV), off.to(DEV))
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(loss.sum(), xd, create_graph=True)
+
+
+def test_training_step_with_the_router(gpu_available):
+    """route's ids, the loss added to another one, gradients through a weight
+    matrix; the bias update's counts."""
+    m = pkg()
+    g = torch.Generator().manual_seed(10)
+    h, w = torch.randn(96, 64, generator=g).to(DEV), (0.2 * torch.randn(256, 64, generator=g)).to(DEV).requires_grad_(True)
+    bias = torch.zeros(256, dtype=torch.bfloat16, device=DEV)
+    logits = h @ w.t()
+    ids, _, n = m.route(logits.detach(), bias, 0, 256, 2.5)
+    off = torch.tensor([0, 40, 96], dtype=torch.int32, device=DEV)
+    loss, counts = m.balance_loss(logits, ids, off, 0.1)
+    assert torch.equal(counts.sum(0, dtype=torch.int32), n)
+    (loss.sum() + logits.square().mean()).backward()
+    wd = w.detach().double().cpu().requires_grad_(True)
+    lg = h.double().cpu() @ wd.t()
+    want, _, back = R.balance(lg, ids.cpu(), off.cpu(), 0.1, "sigmoid")
+    lg.backward(back(torch.ones(2)) + 2 * lg.detach() / lg.numel())
+    # float32 products over 64 columns and 96 rows: 2^-24 (64 + 96) of the sum of magnitudes, a few of the result's size
+    assert ((w.grad.cpu().double() - wd.grad).norm() / wd.grad.norm()) < 160 * 2.0 ** -24 * 8
+
+
 def test_refusals(gpu_available):
     m = pkg()
     x = torch.zeros(8, 16, device=DEV)

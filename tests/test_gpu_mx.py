@@ -260,16 +260,36 @@ def test_matmul_types_alpha_and_strided_output(gpu_available, dtype):
     assert (out[0] == 9).all() and (out[71] == 9).all() and (out[:, :3] == 9).all() and (out[:, 204:] == 9).all()
 
 
-def test_matmul_nan_scale_stays_in_its_row(gpu_available):
+@pytest.mark.parametrize("fmt", FMTS)
+def test_matmul_nan_scale_stays_in_its_row(gpu_available, fmt):
     g = _gen(13)
-    a, sa = R.random_packed(g, (), 40, 512, "mxfp4")
-    b, sb = R.random_packed(g, (), 140, 512, "mxfp4")
-    sa.view(torch.uint8)[7, 3] = 255
-    sb.view(torch.uint8)[131, 9] = 255
-    out = pkg().matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), "mxfp4", out_dtype=torch.float32).cpu()
+    a, sa = R.random_packed(g, (), 40, 512, fmt)
+    b, sb = R.random_packed(g, (), 140, 512, fmt)
+    nan = 0x7F if fmt == "nvfp4" else 255
+    sa.view(torch.uint8)[7, 3] = nan
+    sb.view(torch.uint8)[131, 9] = nan
+    out = pkg().matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), fmt, out_dtype=torch.float32).cpu()
     nan = torch.zeros(40, 140, dtype=torch.bool)
     nan[7] = nan[:, 131] = True
     assert torch.equal(out.isnan(), nan)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("shift", [1, 2, 4, 8])
+@pytest.mark.parametrize("m,n,k", [(9, 70, 256), (150, 300, 416)])
+def test_matmul_scales_at_any_address(gpu_available, fmt, shift, m, n, k):
+    """Contiguous scales that start anywhere in memory, and rows of scales of any length."""
+    g = _gen(m + shift)
+    a, sa = R.random_packed(g, (), m, k, fmt)
+    b, sb = R.random_packed(g, (), n, k, fmt)
+
+    def moved(s):
+        flat = torch.full((s.numel() + shift,), 0x7F, dtype=torch.uint8, device=DEV)
+        flat[shift:] = s.view(torch.uint8).flatten().to(DEV)
+        return flat[shift:].view(s.shape).view(s.dtype)
+
+    out = pkg().matmul_mx(a.to(DEV), moved(sa), b.to(DEV), moved(sb), fmt, out_dtype=torch.float32)
+    _product_ok(out, R.values(a, sa, fmt), R.values(b, sb, fmt), 1.0, torch.float32, f"{fmt} {shift}")
 
 
 def test_matmul_empty(gpu_available):
@@ -309,6 +329,39 @@ def test_experts_matmul(gpu_available, fmt, counts, n, k):
         if c:
             lo = int(off[i])
             _product_ok(out[lo:lo + c], av[lo:lo + c], R.values(b[i], sb[i], fmt), float(al[i]), torch.float32, f"expert {i}")
+
+
+@pytest.mark.parametrize("offsets,runs", [([0, 6, 3, 9], [(0, 6), (6, 6), (6, 9)]), ([-4, 2, 1000, 7], [(0, 2), (2, 12), (12, 12)]),
+                                          ([9, 4, 4, 4], [(9, 9)] * 3)])
+def test_experts_matmul_keeps_bad_offsets_inside(gpu_available, offsets, runs):
+    """Offsets that decrease or leave [0, m] are kept inside and in order."""
+    g = _gen(22)
+    a, sa = R.random_packed(g, (), 12, 96, "mxfp8")
+    b, sb = R.random_packed(g, (3,), 40, 96, "mxfp8")
+    out = torch.full((12, 40), 5.0, device=DEV)
+    off = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    pkg().experts_matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), off, "mxfp8", out=out)
+    assert pkg().device_status() == 0
+    left = torch.ones(12, dtype=torch.bool)
+    av = R.values(a, sa, "mxfp8")
+    for e, (lo, hi) in enumerate(runs):
+        left[lo:hi] = False
+        if lo < hi:
+            _product_ok(out[lo:hi], av[lo:hi], R.values(b[e], sb[e], "mxfp8"), 1.0, torch.float32)
+    assert (out.cpu()[left] == 5).all()
+
+
+def test_experts_matmul_more_experts_than_a_warp_scans(gpu_available):
+    counts = [3 if i % 5 == 0 else 0 for i in range(300)]
+    off, m = _runs(counts)
+    g = _gen(23)
+    a, sa = R.random_packed(g, (), m, 64, "mxfp4")
+    b, sb = R.random_packed(g, (300,), 24, 64, "mxfp4")
+    out = pkg().experts_matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), off.to(DEV), "mxfp4", out_dtype=torch.float32)
+    av = R.values(a, sa, "mxfp4")
+    for i in range(0, 300, 5):
+        lo = int(off[i])
+        _product_ok(out[lo:lo + 3], av[lo:lo + 3], R.values(b[i], sb[i], "mxfp4"), 1.0, torch.float32)
 
 
 def test_experts_matmul_without_out_is_zero_outside(gpu_available):
