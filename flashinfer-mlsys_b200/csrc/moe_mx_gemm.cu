@@ -10,17 +10,18 @@
 // tiles against one narrow token tile, and a run's last tile issues only the
 // columns it has.
 //
-// Warp roles (448 threads, one CTA per SM, persistent):
+// Warp roles (480 threads, one CTA per SM, persistent):
 //   warp 0       TMA producer: 128 bytes of K of the weight tile and of the
 //                token tile per stage (256 4-bit or 128 8-bit values)
-//   warp 1       TMEM owner and MMA issuer: copies the stage's scales to TMEM
-//                (tcgen05.cp) and issues four K slices of 32 bytes
+//   warp 1       TMEM owner and MMA issuer: four K slices of 32 bytes a stage
 //   warps 2-5    scale loaders, four stages at a time. Scales are stored row by
 //                row; the tensor core wants, for 128 rows, word w of row r at
 //                lane r % 32, column r / 32: a lane loads the words of rows
 //                r, r + 32, r + 64, r + 96 and stores them transposed.
 //   warps 6-13   epilogue: TMEM -> registers -> global, two warps a lane quarter
-// TMEM (512 columns): two slots of scales at the top and two accumulators of
+//   warp 14      copies of the stages' scales from shared memory to TMEM
+//                (tcgen05.cp), where the MMA issuer does not do that itself
+// TMEM (512 columns): two or four slots of scales at the top and two accumulators of
 // the tile's width below, which overlap in their middle when two do not fit;
 // the epilogue drains the shared columns first and frees them.
 // Few tiles and a long K: a cluster of up to 8 CTAs splits K, and each adds its
@@ -39,9 +40,10 @@ namespace {
 constexpr int kMxMaxExperts = kMxGemmMaxExperts;
 constexpr int kMxTileN = 128;     // weight rows of a tile
 constexpr int kMxStageK = 128;    // bytes of K of a stage
-constexpr int kMxGemmThreads = 448;
+constexpr int kMxGemmThreads = 480;
 constexpr int kMxSfWarp0 = 2, kMxSfWarps = 4;
 constexpr int kMxEpiWarp0 = 6, kMxEpiWarps = 8;
+constexpr int kMxCopyWarp = 14;
 constexpr uint64_t kMxWaitNs = 2000000000ull;  // 2 s: only reached if something is broken
 
 __device__ unsigned g_mx_status;  // kErrTimeout if a bounded wait gave up
@@ -57,7 +59,15 @@ struct MxCfg {
   static constexpr int kGroupBytes = 4 * kSfBytes;  // scales of four stages
   static constexpr int kGroups = kPair ? (kW > 2 ? 3 : 4) : 2;  // slots of them
   static constexpr int kSfCols = kW * 4 * (1 + kChunks);  // TMEM columns of one slot
-  static constexpr int kAccCols = (512 - 2 * kSfCols) & ~31;
+  // The copies of scales to TMEM are issued by a warp of their own, up to four
+  // stages ahead; among the MMAs, one warp's issue took 450 of the 950 cycles of
+  // a stage. Not so for pairs with nvfp4, whose twelve copies a stage slow the
+  // MMAs down when they run ahead of them. Measured, copies apart / in line:
+  // experts' nvfp4 products of 64 rows 73.9 / 79.2 us, 8192 x 7168 x 4096 mxfp4
+  // 95.8 / 97.3 us, mxfp8 182.8 / 184.5 us, nvfp4 112.8 / 107.0 us.
+  static constexpr bool kCopyApart = !kPair || kW < 4;
+  static constexpr int kSlots = kCopyApart ? 4 : 2;
+  static constexpr int kAccCols = (512 - kSlots * kSfCols) & ~31;
   // 16-column pieces of the overlap of two widest accumulators that a warp of the epilogue holds
   static constexpr int kShared = kNT - ((kAccCols - kNT) & ~31);
   static constexpr int kHeld = kShared > 0 ? (kShared / 16 + 1) / 2 : 0;
@@ -85,7 +95,7 @@ struct MxGemmArgs {
 };
 
 struct __align__(16) MxCtl {
-  uint64_t full[8], empty[8], sf_full[4], sf_empty[4], peer_sf[4], tfull[2], acc_free, peer_acc, part_ready, part_free, mma_done;
+  uint64_t full[8], empty[8], sf_full[4], sf_empty[4], peer_sf[4], cp_full[4], tfull[2], acc_free, peer_acc, part_ready, part_free, mma_done, cp_done;
   uint32_t tmem_base;
   int abort_flag;
   int start[kMxMaxExperts + 1];   // first row of each run
@@ -187,6 +197,15 @@ __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint3
   }
 }
 #undef MX_MMA
+
+// The same on this CTA's barrier alone.
+template <bool kPair>
+__device__ __forceinline__ void mx_commit_own(uint64_t* bar) {
+  if constexpr (kPair)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  else
+    mma_commit(bar);
+}
 
 // Arrive on `bar` (of both CTAs of a pair) once this thread's earlier MMAs and copies are done.
 template <bool kPair>
@@ -385,6 +404,8 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     mbar_init(&ctl->part_ready, p.split);
     mbar_init(&ctl->part_free, p.split);
     mbar_init(&ctl->mma_done, 1);
+    mbar_init(&ctl->cp_done, 1);
+    for (int b = 0; b < Cfg::kSlots; ++b) mbar_init(&ctl->cp_full[b], 1);
     ctl->abort_flag = 0;
     fence_barrier_init();
     prefetch_tensormap(&map_w);
@@ -450,6 +471,30 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   const uint32_t acc_at[2] = {tmem, tmem + acc1};
   const uint32_t sf_at = tmem + Cfg::kAccCols;
 
+  // Issues the copies of a stage's scales (stage kg of group slot gs) to TMEM slot `slot`.
+  const auto copy_scales = [&](uint32_t gs, int kg, uint32_t slot, int cnt) {
+    const uint32_t sf = smem_u32(sfs + gs * Cfg::kGroupBytes + kg * Cfg::kSfBytes);
+    const uint32_t t_w = sf_at + slot * Cfg::kSfCols, t_a = t_w + 4 * kW;
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      tmem_cp_sf<kPair>(t_w + 4 * i, sf + i * 512);
+#pragma unroll
+      for (int c = 0; c < Cfg::kChunks; ++c)
+        if (c * 128 < cnt)
+          tmem_cp_sf<kPair>(t_a + (i * Cfg::kChunks + c) * 4, sf + kW * 512 + (i * Cfg::kChunks + c) * 512);
+    }
+  };
+  // Waits for the scales of group `grp` and, from the kSlots-th stage on, for
+  // the TMEM slot of stage `it` (its last readers: the MMAs kSlots stages back).
+  const auto copy_ready = [&](uint32_t it, uint32_t grp, bool first) {
+    bool ok = true;
+    if (first)
+      ok = mx_wait_both<kPair>(&ctl->sf_full[grp % Cfg::kGroups], &ctl->peer_sf[grp % Cfg::kGroups], (grp / Cfg::kGroups) & 1u);
+    if (ok && it >= Cfg::kSlots)
+      ok = mbar_wait_bounded(&ctl->empty[(it - Cfg::kSlots) % kS], ((it - Cfg::kSlots) / kS) & 1u, kMxWaitNs);
+    return all_lanes(ok);
+  };
+
   if (warp == 0) {
     // ======================= TMA producer =======================
     if (lane == 0) {
@@ -496,7 +541,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   } else if (warp == 1) {
     // ======================= MMA issuer =======================
     // The whole warp walks the loop and one elected lane issues: with every
-    // operand the same in all lanes an issue costs a few cycles, where a
+    // operand the same in all lanes an issue costs some 25 cycles, where a
     // branch on the lane cost some 70 for each (182 -> 145 us at 8192 x 7168 x 4096 nvfp4).
     if (!kPair || rank == 0) {
       uint32_t it = 0, tile = 0, grp = 0;
@@ -512,27 +557,18 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         }
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % kS, kg = (k - k0) & 3;
-          const uint32_t gs = grp % Cfg::kGroups;
-          if (kg == 0 && !all_lanes(mx_wait_both<kPair>(&ctl->sf_full[gs], &ctl->peer_sf[gs], (grp / Cfg::kGroups) & 1u))) {
-            mx_abort(ctl);
-            break;
-          }
-          // the TMEM scale slot's last readers have finished (two stages back)
-          if (it >= 2 && !all_lanes(mbar_wait_bounded(&ctl->empty[(it - 2) % kS], ((it - 2) / kS) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
-          if (!all_lanes(mbar_wait_bounded(&ctl->full[s], (it / kS) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
-          tc_fence_after();
           const bool group_ends = kg == 3 || k == k1 - 1;
+          if constexpr (!Cfg::kCopyApart) {
+            if (!copy_ready(it, grp, kg == 0)) { mx_abort(ctl); break; }
+          }
+          bool ok = mbar_wait_bounded(&ctl->full[s], (it / kS) & 1u, kMxWaitNs);
+          if constexpr (Cfg::kCopyApart)
+            ok = ok && mbar_wait_bounded(&ctl->cp_full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1u, kMxWaitNs);
+          if (!all_lanes(ok)) { mx_abort(ctl); break; }
+          tc_fence_after();
           if (el) {
-            const uint32_t sf = smem_u32(sfs + gs * Cfg::kGroupBytes + kg * Cfg::kSfBytes);
-            const uint32_t t_w = sf_at + (it & 1u) * Cfg::kSfCols, t_a = t_w + 4 * kW;
-#pragma unroll
-            for (int i = 0; i < kW; ++i) {
-              tmem_cp_sf<kPair>(t_w + 4 * i, sf + i * 512);
-#pragma unroll
-              for (int c = 0; c < Cfg::kChunks; ++c)
-                if (c * 128 < nmma)
-                  tmem_cp_sf<kPair>(t_a + (i * Cfg::kChunks + c) * 4, sf + kW * 512 + (i * Cfg::kChunks + c) * 512);
-            }
+            if constexpr (!Cfg::kCopyApart) copy_scales(grp % Cfg::kGroups, kg, it % Cfg::kSlots, x.cnt);
+            const uint32_t t_w = sf_at + (it % Cfg::kSlots) * Cfg::kSfCols, t_a = t_w + 4 * kW;
             const uint32_t st = smem_u32(tiles + s * Cfg::kStageBytes);
             const uint64_t dw = smem_desc_sw128(st), da = smem_desc_sw128(st + Cfg::kTileBytes);
 #pragma unroll
@@ -544,7 +580,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
                                   t_a + word * Cfg::kChunks * 4, (k > k0 || j > 0) ? 1u : 0u);
             }
             mx_commit<kPair>(&ctl->empty[s]);
-            if (group_ends) mx_commit<kPair>(&ctl->sf_empty[gs]);
+            if (!Cfg::kCopyApart && group_ends) mx_commit<kPair>(&ctl->sf_empty[grp % Cfg::kGroups]);
           }
           __syncwarp();
           if (group_ends) ++grp;
@@ -663,6 +699,32 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       loop(std::integral_constant<int, 4>{});
     else
       loop(std::integral_constant<int, 1>{});
+  } else if (warp == kMxCopyWarp) {
+    // ======================= scale copies to TMEM =======================
+    if (Cfg::kCopyApart && (!kPair || rank == 0)) {
+      uint32_t it = 0, grp = 0;
+      const bool el = elect_one();
+      for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
+        const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int kg = (k - k0) & 3;
+          const bool group_ends = kg == 3 || k == k1 - 1;
+          if (!copy_ready(it, grp, kg == 0)) { mx_abort(ctl); break; }
+          tc_fence_after();
+          if (el) {
+            copy_scales(grp % Cfg::kGroups, kg, it % Cfg::kSlots, x.cnt);
+            mx_commit_own<kPair>(&ctl->cp_full[it % Cfg::kSlots]);
+            if (group_ends) mx_commit<kPair>(&ctl->sf_empty[grp % Cfg::kGroups]);
+          }
+          __syncwarp();
+          if (group_ends) ++grp;
+        }
+      }
+      if (mx_aborted(ctl) && it > 0) {
+        if (el) mx_commit<kPair>(&ctl->cp_done);
+        mbar_wait_bounded(&ctl->cp_done, 0, kMxWaitNs);
+      }
+    }
   } else {
     // ======================= epilogue (8 warps) =======================
     const int q = warp & 3, half = (warp - kMxEpiWarp0) >> 2;
