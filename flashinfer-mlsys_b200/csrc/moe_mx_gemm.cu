@@ -55,7 +55,7 @@ struct MxCfg {
   static constexpr int kTileBytes = kMxTileN * kMxStageK;
   static constexpr int kStageBytes = kTileBytes + (kPair ? kNT / 2 : kNT) * kMxStageK;  // a pair halves the tokens
   static constexpr int kSfBytes = kW * 512 * (1 + kChunks);
-  static constexpr int kStages = kPair ? 4 : (kNT > 64 ? 5 : (kNT > 32 ? 6 : 8));
+  static constexpr int kStages = kPair ? (kW > 2 ? 4 : 5) : (kNT > 64 ? 5 : (kNT > 32 ? 6 : 8));
   static constexpr int kGroupBytes = 4 * kSfBytes;  // scales of four stages
   static constexpr int kGroups = kPair ? (kW > 2 ? 3 : 4) : 2;  // slots of them
   static constexpr int kSfCols = kW * 4 * (1 + kChunks);  // TMEM columns of one slot
@@ -497,8 +497,15 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 
   if (warp == 0) {
     // ======================= TMA producer =======================
-    if (lane == 0) {
-      uint32_t it = 0;
+    // The whole warp walks the loop and one elected lane issues (see the MMA
+    // issuer); from a branch on the lane a copy takes some 200 cycles. Where the
+    // MMA issuer is the slower one all the same, one lane does better: 8192 x
+    // 7168 x 4096 nvfp4 107.3 against 110.9 us, mxfp8 182.6 against 174.2 us,
+    // 1000 x 2048 x 7168 mxfp8 19.8 against 18.7 us.
+    constexpr bool kWhole = Cfg::kCopyApart;
+    uint32_t it = 0;
+    const bool el = kWhole ? elect_one() : lane == 0;
+    if (kWhole || el) {
       for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
         const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
         // token rows of this CTA: the columns that are issued, of which the
@@ -509,33 +516,38 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         const uint32_t bytes = Cfg::kTileBytes + boxes * p.box * kMxStageK;
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % kS;
-          if (!mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs)) { mx_abort(ctl); break; }
-          uint8_t* st = tiles + s * Cfg::kStageBytes;
-          if constexpr (kPair) {
-            // both CTAs' copies count on the first CTA's barrier
-            const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
-            if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * bytes);
-            tma_load_3d_pair(st, &map_w, k * kMxStageK, x.n0 + my_n, x.e, bar);
-            for (int b = 0; b < boxes; ++b)
-              tma_load_3d_pair(st + Cfg::kTileBytes + b * p.box * kMxStageK, &map_a, k * kMxStageK, row_a + b * p.box, 0, bar);
-          } else {
-            mbar_arrive_expect_tx(&ctl->full[s], bytes);
-            tma_load_3d(st, &map_w, k * kMxStageK, x.n0, x.e, &ctl->full[s]);
-            for (int b = 0; b < boxes; ++b)
-              tma_load_3d(st + Cfg::kTileBytes + b * p.box * kMxStageK, &map_a, k * kMxStageK, row_a + b * p.box, 0, &ctl->full[s]);
+          bool ok = mbar_wait_bounded(&ctl->empty[s], ((it / kS) & 1u) ^ 1u, kMxWaitNs);
+          if (kWhole) ok = all_lanes(ok);
+          if (!ok) { mx_abort(ctl); break; }
+          if (el) {
+            uint8_t* st = tiles + s * Cfg::kStageBytes;
+            if constexpr (kPair) {
+              // both CTAs' copies count on the first CTA's barrier
+              const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
+              if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * bytes);
+              tma_load_3d_pair(st, &map_w, k * kMxStageK, x.n0 + my_n, x.e, bar);
+              for (int b = 0; b < boxes; ++b)
+                tma_load_3d_pair(st + Cfg::kTileBytes + b * p.box * kMxStageK, &map_a, k * kMxStageK, row_a + b * p.box, 0, bar);
+            } else {
+              mbar_arrive_expect_tx(&ctl->full[s], bytes);
+              tma_load_3d(st, &map_w, k * kMxStageK, x.n0, x.e, &ctl->full[s]);
+              for (int b = 0; b < boxes; ++b)
+                tma_load_3d(st + Cfg::kTileBytes + b * p.box * kMxStageK, &map_a, k * kMxStageK, row_a + b * p.box, 0, &ctl->full[s]);
+            }
           }
+          if (kWhole) __syncwarp();
         }
       }
-      if (mx_aborted(ctl)) {
-        // wait (bounded) for the copies in flight; the second CTA of a pair,
-        // whose copies count elsewhere, gives them a millisecond
-        if (rank == 0 || !kPair) {
-          for (uint32_t j = it > (uint32_t)kS ? it - kS : 0; j < it; ++j)
-            mbar_wait_bounded(&ctl->full[j % kS], (j / kS) & 1u, kMxWaitNs);
-        } else {
-          const uint64_t t0 = global_timer_ns();
-          while (global_timer_ns() - t0 < 1000000) __nanosleep(1000);
-        }
+    }
+    if (mx_aborted(ctl) && el) {
+      // wait (bounded) for the copies in flight; the second CTA of a pair,
+      // whose copies count elsewhere, gives them a millisecond
+      if (rank == 0 || !kPair) {
+        for (uint32_t j = it > (uint32_t)kS ? it - kS : 0; j < it; ++j)
+          mbar_wait_bounded(&ctl->full[j % kS], (j / kS) & 1u, kMxWaitNs);
+      } else {
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000) __nanosleep(1000);
       }
     }
   } else if (warp == 1) {
@@ -623,73 +635,73 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     const uint8_t* end_a = p.sa + static_cast<int64_t>(p.R) * p.nsc;
     // one loop for each kind of row, so that there are no branches among the loads
     const auto loop = [&](auto align) {
-    constexpr int kA = decltype(align)::value;  // bytes of a load; 1: words around the bytes
-    constexpr int kR = kA > 1 ? kW : kW + 1;    // words held of a row and stage
-    const int64_t ld = p.nsc;
-    // the words of stages k .. k + 3 of unit x: 128-row group g = 0 is the
-    // weights', the others the tokens'
-    const auto load = [&](const MxUnit& x, int k, uint32_t (&w)[1 + Cfg::kChunks][4][kR]) {
-      const int n0 = x.n0 + my_n;
-      const int at = (k + j) * 4 * kW;
-      const int left = k + j < k1 ? p.nsc - at : 0;
-      const uint8_t* base[2] = {p.sw + (static_cast<int64_t>(x.e) * p.N + n0) * ld, p.sa + x.row0 * ld};
-      bool inside = true;
-      if constexpr (kA == 1) {
-        // the four stages' words of the last row of either side
-        const int64_t last = static_cast<int64_t>(k + 4) * 4 * kW + 4;
-        inside = (reinterpret_cast<uint64_t>(p.sw) & 3) == 0 && (reinterpret_cast<uint64_t>(p.sa) & 3) == 0 &&
-                 base[0] + (min(kMxTileN, p.N - n0) - 1) * ld + last <= end_w && base[1] + (x.cnt - 1) * ld + last <= end_a;
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int g = 0; g <= Cfg::kChunks; ++g) {
-          const int r = r0 + 32 * q + (g > 1 ? 128 : 0);
-          const int mine = r < (g == 0 ? p.N - n0 : x.cnt) ? left : 0;
-          const uint8_t* s = base[g > 0] + r * ld + at;
-          if constexpr (kA > 1)
-            mx_sf_aligned<kW, kA>(s, mine, g == 0 ? p.sw : p.sa, w[g][q]);
-          else
-            mx_sf_around<kW>(s, mine, inside, g == 0 ? p.sw : p.sa, g == 0 ? end_w : end_a, w[g][q]);
+      constexpr int kA = decltype(align)::value;  // bytes of a load; 1: words around the bytes
+      constexpr int kR = kA > 1 ? kW : kW + 1;    // words held of a row and stage
+      const int64_t ld = p.nsc;
+      // the words of stages k .. k + 3 of unit x: 128-row group g = 0 is the
+      // weights', the others the tokens'
+      const auto load = [&](const MxUnit& x, int k, uint32_t (&w)[1 + Cfg::kChunks][4][kR]) {
+        const int n0 = x.n0 + my_n;
+        const int at = (k + j) * 4 * kW;
+        const int left = k + j < k1 ? p.nsc - at : 0;
+        const uint8_t* base[2] = {p.sw + (static_cast<int64_t>(x.e) * p.N + n0) * ld, p.sa + x.row0 * ld};
+        bool inside = true;
+        if constexpr (kA == 1) {
+          // the four stages' words of the last row of either side
+          const int64_t last = static_cast<int64_t>(k + 4) * 4 * kW + 4;
+          inside = (reinterpret_cast<uint64_t>(p.sw) & 3) == 0 && (reinterpret_cast<uint64_t>(p.sa) & 3) == 0 &&
+                   base[0] + (min(kMxTileN, p.N - n0) - 1) * ld + last <= end_w && base[1] + (x.cnt - 1) * ld + last <= end_a;
         }
-      }
-    };
-    // word i of row q of group g, of the stage that this lane loaded
-    const auto word = [&](const MxUnit& x, int k, const uint32_t (&w)[1 + Cfg::kChunks][4][kR], int g, int q, int i) {
-      if constexpr (kA == 4 * kW) return w[g][q][i];
-      const int r = r0 + 32 * q + (g > 1 ? 128 : 0), at = (k + j) * 4 * kW;
-      const int left = k + j < k1 && r < (g == 0 ? p.N - x.n0 - my_n : x.cnt) ? p.nsc - at : 0;
-      if constexpr (kA > 1) {
-        return 4 * i < left ? w[g][q][i] : 0u;
-      } else {
-        const uint8_t* b = g == 0 ? p.sw + (static_cast<int64_t>(x.e) * p.N + x.n0 + my_n) * ld : p.sa + x.row0 * ld;
-        return mx_sf_shift(w[g][q], i, static_cast<int>((reinterpret_cast<uint64_t>(b) + r * ld + at) & 3u), left);
-      }
-    };
-    uint32_t w[1 + Cfg::kChunks][4][kR];
-    uint32_t grp = 0;
-    for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
-      const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
-      bool ok = true;
-      for (int k = k0; k < k1; k += 4, ++grp) {
-        load(x, k, w);  // under way while the slot is still being read
-        const uint32_t gs = grp % Cfg::kGroups;
-        ok = all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp / Cfg::kGroups) & 1u) ^ 1u, kMxWaitNs));
-        if (!ok) break;
-        uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
 #pragma unroll
-        for (int i = 0; i < kW; ++i) {
+        for (int q = 0; q < 4; ++q) {
 #pragma unroll
-          for (int g = 0; g <= Cfg::kChunks; ++g)
-            *reinterpret_cast<uint4*>(sf + (g == 0 ? i : kW + i * Cfg::kChunks + g - 1) * 512) =
-                make_uint4(word(x, k, w, g, 0, i), word(x, k, w, g, 1, i), word(x, k, w, g, 2, i), word(x, k, w, g, 3, i));
+          for (int g = 0; g <= Cfg::kChunks; ++g) {
+            const int r = r0 + 32 * q + (g > 1 ? 128 : 0);
+            const int mine = r < (g == 0 ? p.N - n0 : x.cnt) ? left : 0;
+            const uint8_t* s = base[g > 0] + r * ld + at;
+            if constexpr (kA > 1)
+              mx_sf_aligned<kW, kA>(s, mine, g == 0 ? p.sw : p.sa, w[g][q]);
+            else
+              mx_sf_around<kW>(s, mine, inside, g == 0 ? p.sw : p.sa, g == 0 ? end_w : end_a, w[g][q]);
+          }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->sf_full[gs]);
+      };
+      // word i of row q of group g, of the stage that this lane loaded
+      const auto word = [&](const MxUnit& x, int k, const uint32_t (&w)[1 + Cfg::kChunks][4][kR], int g, int q, int i) {
+        if constexpr (kA == 4 * kW) return w[g][q][i];
+        const int r = r0 + 32 * q + (g > 1 ? 128 : 0), at = (k + j) * 4 * kW;
+        const int left = k + j < k1 && r < (g == 0 ? p.N - x.n0 - my_n : x.cnt) ? p.nsc - at : 0;
+        if constexpr (kA > 1) {
+          return 4 * i < left ? w[g][q][i] : 0u;
+        } else {
+          const uint8_t* b = g == 0 ? p.sw + (static_cast<int64_t>(x.e) * p.N + x.n0 + my_n) * ld : p.sa + x.row0 * ld;
+          return mx_sf_shift(w[g][q], i, static_cast<int>((reinterpret_cast<uint64_t>(b) + r * ld + at) & 3u), left);
+        }
+      };
+      uint32_t w[1 + Cfg::kChunks][4][kR];
+      uint32_t grp = 0;
+      for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
+        const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+        bool ok = true;
+        for (int k = k0; k < k1; k += 4, ++grp) {
+          load(x, k, w);  // under way while the slot is still being read
+          const uint32_t gs = grp % Cfg::kGroups;
+          ok = all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp / Cfg::kGroups) & 1u) ^ 1u, kMxWaitNs));
+          if (!ok) break;
+          uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
+#pragma unroll
+          for (int i = 0; i < kW; ++i) {
+#pragma unroll
+            for (int g = 0; g <= Cfg::kChunks; ++g)
+              *reinterpret_cast<uint4*>(sf + (g == 0 ? i : kW + i * Cfg::kChunks + g - 1) * 512) =
+                  make_uint4(word(x, k, w, g, 0, i), word(x, k, w, g, 1, i), word(x, k, w, g, 2, i), word(x, k, w, g, 3, i));
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->sf_full[gs]);
+        }
+        if (!ok) { mx_abort(ctl); break; }
       }
-      if (!ok) { mx_abort(ctl); break; }
-    }
     };
     if (kW == 4 && (low & 15) == 0)
       loop(std::integral_constant<int, kW == 4 ? 16 : 4>{});
