@@ -7,6 +7,7 @@ It links the CUDA runtime statically and resolves the driver entry point
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -56,16 +57,19 @@ def build(force: bool = False, verbose: bool = False) -> str:
     nvcc = _nvcc()
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
-    for src in SOURCES:
-        obj = os.path.join(objdir, src.replace(".cu", ".o"))
-        cmd = [nvcc, *NVCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
-        r = subprocess.run(cmd, capture_output=True, text=True)
+    objs = [os.path.join(objdir, src.replace(".cu", ".o")) for src in SOURCES]
+
+    def compile_one(job):
+        src, obj = job
+        return subprocess.run([nvcc, *NVCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj], capture_output=True, text=True)
+
+    with concurrent.futures.ThreadPoolExecutor(min(4, os.cpu_count() or 1)) as pool:
+        results = list(pool.map(compile_one, zip(SOURCES, objs)))
+    for src, r in zip(SOURCES, results):
         if verbose or r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed on {src}")
-        objs.append(obj)
     tmp = LIB_PATH + ".tmp"
     cmd = [nvcc, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

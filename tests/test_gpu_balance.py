@@ -155,6 +155,41 @@ def test_empty_repeat_graph_and_backward_twice(gpu_available):
     assert torch.equal(cg.cpu().long(), n)
 
 
+def test_forward_and_backward_in_a_graph(gpu_available):
+    """The whole step captured, replayed on new logits; a call on another
+    stream meanwhile, with a workspace of its own."""
+    m = pkg()
+    x, ids, off, grad = _inputs(700, 256, 8, 5, torch.float32, 12)
+    idd, offd, gd = ids.to(DEV), off.to(DEV), grad.to(DEV)
+    xs = x.to(DEV).requires_grad_(True)
+
+    def step():
+        loss, _ = m.balance_loss(xs, idd, offd, 0.5, "softmax")
+        return loss, torch.autograd.grad(loss, xs, gd)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, dx = step()
+    y = (0.3 * x).to(DEV)
+    with torch.no_grad():
+        xs.copy_(y)
+    torch.cuda.synchronize()
+    graph.replay()
+    with torch.cuda.stream(side):
+        other = [m.balance_loss(y, idd, offd, 0.5, "softmax")[0] for _ in range(20)]
+    torch.cuda.synchronize()
+    want, _, back = R.balance(0.3 * x, ids, off, 0.5, "softmax")
+    torch.testing.assert_close(loss.detach().cpu().double(), want, rtol=2.0 ** -16, atol=0)
+    assert all(torch.equal(o, loss) for o in other)
+    ref = back(grad)
+    assert (dx.cpu().double() - ref).norm() <= 2.0 ** -16 * ref.norm()
+
+
 def test_second_derivative_is_refused(gpu_available):
     x, ids, off, _ = _inputs(8, 16, 2, 1, torch.float32, 9)
     xd = x.to(DEV).requires_grad_(True)

@@ -110,6 +110,28 @@ def test_quantize_strides_outputs_and_empty(gpu_available):
         assert m.add_rmsnorm_quantize_mx(e, e.clone(), None, fmt=fmt)[0].shape[0] == 0
 
 
+def test_more_than_2_31_elements(gpu_available):
+    """Rows whose offsets pass 32 bits, in and out (about 10 GB)."""
+    m = pkg()
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB of free device memory")
+    rows, cols = 310000, 7168
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[:2], x[-2:] = 1.0, _hidden(2, cols, torch.bfloat16, 6).to(DEV)
+    q, s = m.quantize_mx(x, "mxfp4")
+    _quantised("mxfp4", q[-2:], s[-2:], x[-2:].cpu())
+    m.dequantize_mx(q, s, "mxfp4", out=x)
+    assert torch.equal(x[-2:].cpu(), R.values(q[-2:].cpu(), s[-2:].cpu(), "mxfp4").bfloat16())
+    b, sb = R.random_packed(_gen(7), (), cols, 32, "mxfp8")
+    a = torch.zeros(rows, 32, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    sa = torch.full((rows, 1), 127, dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    last, _ = R.random_packed(_gen(8), (), 2, 32, "mxfp8")
+    a.view(torch.uint8)[-2:] = last.view(torch.uint8).to(DEV)
+    m.matmul_mx(a, sa, b.to(DEV), sb.to(DEV), "mxfp8", out=x)
+    assert (x[:-2:50000] == 0).all() and m.device_status() == 0
+    _product_ok(x[-2:], last.double(), R.values(b, sb, "mxfp8"), 1.0, torch.bfloat16)
+
+
 def test_refusals_on_the_device(gpu_available):
     m = pkg()
     x = torch.zeros(4, 64, device=DEV, dtype=torch.bfloat16)
@@ -177,6 +199,28 @@ def test_norm(gpu_available, fmt, dtype, rows, cols):
     h = h.double()
     y = h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-5) * w.double()
     _check_rows(fmt, q, s, y)
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+def test_norm_rounds_the_exact_value(gpu_available, dtype):
+    """mxfp8 values and scales are those of the exact y (float64), rounded once:
+    the sum's error of some 2^-30 moves one value in 10^8 across a border."""
+    dt = R.DTYPES[dtype]
+    g = _gen(77)
+    x, w = torch.randn(40, 7168, generator=g).to(dt), (1 + 0.2 * torch.randn(7168, generator=g)).to(dt)
+    x[3] = 1.0
+    x[4] = 0.0
+    w[:64] = 1.0
+    q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, w.to(DEV), 2.0 ** -20, "mxfp8")
+    h = x.double()
+    y = h * w.double() / torch.sqrt(h.square().mean(1, keepdim=True) + 2.0 ** -20)
+    amax = y.abs().view(40, -1, 32).amax(-1)
+    e = torch.where(amax > 0, torch.floor(torch.log2(amax)) - 8 + 127, 0).clamp(0, 254)
+    assert torch.equal(s.view(torch.uint8).cpu().double(), e)
+    t = y / 2.0 ** (e - 127).repeat_interleave(32, 1)
+    ulp = 2.0 ** (torch.floor(torch.log2(t.abs().clamp(min=2.0 ** -6))) - 3)
+    want = (torch.round(t / ulp) * ulp).clamp(-448, 448)
+    assert torch.equal(q.cpu().double(), want)
 
 
 def test_norm_without_residual_or_weight(gpu_available):
