@@ -36,7 +36,7 @@
 //   32 experts x 7168 x 4096 nvfp4, 64 rows   74 us, 6.0 TB/s: HBM
 //   32 experts x 2048 x 7168 mxfp4, 8192 rows 88 us, 4.3 TB/s: eight stages a
 //     tile, in which neither HBM (55%) nor the tensor pipe (34%) is kept busy
-//   8 x 7168 x 4096 nvfp4       7.6 us: launch, one exchange across the
+//   8 x 7168 x 4096 nvfp4       7.2 us: launch, one exchange across the
 //     cluster and some 2.6 us of weights
 #include <atomic>
 #include <type_traits>
@@ -82,11 +82,10 @@ struct MxCfg {
   // 16-column pieces of the overlap of two widest accumulators that a warp of the epilogue holds
   static constexpr int kShared = kNT - ((kAccCols - kNT) & ~31);
   static constexpr int kHeld = kShared > 0 ? (kShared / 16 + 1) / 2 : 0;
-  static constexpr bool kOwnPart = kNT <= 64;             // room for the split's partial sums beside the ring
+  // a split's partial sums take the ring's place: its cluster has one tile, whose stages are used up by then
   static constexpr int kPartBytes = kNT * kMxTileN * 4;
-  static constexpr size_t kSmem =
-      1024 + (size_t)kStages * kStageBytes + kGroups * kGroupBytes + (kOwnPart ? kPartBytes : 0);
-  static_assert(kOwnPart || kPartBytes <= kStages * kStageBytes, "partial sums reuse the ring");
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kGroups * kGroupBytes;
+  static_assert(kPair || kPartBytes <= kStages * kStageBytes, "partial sums reuse the ring");
   static_assert(kSlots <= kStages, "the readers of a TMEM slot are known by the ring stage they free");
 };
 
@@ -111,7 +110,7 @@ struct __align__(16) MxCtl {
   uint64_t sf_full[4], sf_empty[4], peer_sf[4];    // groups of scales; peer_sf: the second CTA's, by its relay
   uint64_t cp_full[4];                             // scales in TMEM
   uint64_t tfull[2], acc_free, peer_acc;           // accumulators
-  uint64_t part_ready, part_free;                  // a split's partial sums
+  uint64_t part_ready;                             // a split's partial sums
   uint64_t mma_done, cp_done;                      // after a wait that gave up
   uint32_t tmem_base;
   int abort_flag;
@@ -389,7 +388,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   MxCtl* ctl = &ctl_;
   uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sfs = tiles + kS * Cfg::kStageBytes;
-  float* part = reinterpret_cast<float*>(Cfg::kOwnPart ? sfs + Cfg::kGroups * Cfg::kGroupBytes : tiles);
+  float* part = reinterpret_cast<float*>(tiles);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // a unit is one tile of weight rows x tokens, and belongs to a cluster: a
@@ -419,7 +418,6 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     mbar_init(&ctl->acc_free, kMxEpiWarps);
     mbar_init(&ctl->peer_acc, kMxEpiWarps);
     mbar_init(&ctl->part_ready, p.split);
-    mbar_init(&ctl->part_free, p.split);
     mbar_init(&ctl->mma_done, 1);
     mbar_init(&ctl->cp_done, 1);
     for (int b = 0; b < Cfg::kSlots; ++b) mbar_init(&ctl->cp_full[b], 1);
@@ -768,9 +766,6 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
       const uint32_t buf = tile & 1u;
       const float alpha = p.alpha ? __ldg(p.alpha + x.e) : 1.0f;
-      if (p.split > 1 && tile > 0) {  // the cluster has read this CTA's last partial sums
-        if (!all_lanes(cluster_wait_bounded(&ctl->part_free, (tile - 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
-      }
       if (!all_lanes(mbar_wait_bounded(&ctl->tfull[buf], (tile >> 1) & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
       __syncwarp();
       tc_fence_after();
@@ -816,7 +811,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (p.split > 1) {
         epi_bar_sync();
         if (etid < p.split) cluster_arrive_remote(cluster_map(smem_u32(&ctl->part_ready), etid));
-        if (!all_lanes(cluster_wait_bounded(&ctl->part_ready, tile & 1u, kMxWaitNs))) { mx_abort(ctl); break; }
+        if (!all_lanes(cluster_wait_bounded(&ctl->part_ready, 0, kMxWaitNs))) { mx_abort(ctl); break; }
         // tokens rank, rank + split, ...: a warp a token, four weight rows a lane
         const int n = x.n0 + lane * 4;
         for (int t = rank + (warp - kMxEpiWarp0) * p.split; t < x.cnt; t += kMxEpiWarps * p.split) {
@@ -832,8 +827,6 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
           if (n + 2 < p.N) mx_out_store(p, row, n + 2, sum.z * alpha);
           if (n + 3 < p.N) mx_out_store(p, row, n + 3, sum.w * alpha);
         }
-        epi_bar_sync();
-        if (etid < p.split) cluster_arrive_remote(cluster_map(smem_u32(&ctl->part_free), etid));
       }
     }
   }
@@ -923,8 +916,8 @@ MxPlan mx_gemm_plan(int64_t rows, int64_t N, int experts, int nk, bool runs) {
   };
   const auto split_of = [&](int tn) {
     int split = 1;
-    // a cluster with several tiles needs its own room for partial sums (up to 64 tokens)
-    if (tn <= (runs ? 64 : 128))
+    // no pairs, and a tile for every cluster: the exchange is over when the kernel ends
+    if (tn <= 128)
       while (split < 8 && tiles_of(tn) * split * 2 <= sms && nk >= 4 * split) split *= 2;
     return split;
   };
