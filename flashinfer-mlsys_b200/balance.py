@@ -76,7 +76,7 @@ def balance_loss(routing_logits: torch.Tensor, topk_ids: torch.Tensor, seq_offse
 
     Returns (loss float32 [S], counts int32 [S, E]). An empty sequence has loss
     0; tokens of no sequence count nowhere and get a zero gradient; a token
-    whose scores sum to zero in float32 has p = 0. ``counts.sum(0)`` is what a
+    whose scores vanish in float32 (sigmoids of logits under -87) has p = 0. ``counts.sum(0)`` is what a
     bias update of the no-aux router needs."""
     dev = _cuda(routing_logits, "routing_logits")
     _cuda(topk_ids, "topk_ids")

@@ -341,7 +341,7 @@ int moe_fp8_ds_experts_matmul_mx(const void* a, const void* a_scale, const void*
  *   loss_out[s] = coeff * sum_i f_i * mean_t p_ti      (0 for an empty sequence)
  *   counts_out int32 [seqs][experts]: slots of the sequence with that id
  * Ids outside [0, experts) are not counted; an id that occurs twice counts
- * twice. A token whose scores sum to zero in float32 has p = 0.
+ * twice. A token whose scores vanish in float32 has p = 0.
  * logits [tokens][experts] of dtype, rows logits_ld apart; topk_ids int32
  * [tokens][topk]; work: device scratch of moe_fp8_ds_balance_loss_work_bytes
  * bytes, any content. The backward call writes

@@ -416,6 +416,67 @@ def test_experts_matmul_without_out_is_zero_outside(gpu_available):
     assert out.dtype == torch.bfloat16 and (out[:2] == 0).all() and (out[4:] == 0).all() and (out[2:4] != 0).any()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k", [(3, 130, 1 << 20), (130, 130, 1 << 17), (2, 1 << 18, 32), (200, 1 << 18, 32)])
+def test_matmul_longest_axes(gpu_available, fmt, m, n, k):
+    g = _gen(n + m)
+    a, sa = R.random_packed(g, (), m, k, fmt)
+    b, sb = R.random_packed(g, (), n, k, fmt)
+    out = pkg().matmul_mx(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), fmt, out_dtype=torch.float32)
+    assert pkg().device_status() == 0
+    pick = slice(None) if n < 1000 else slice(None, None, 997)
+    av = R.values(a, sa, fmt)
+    _product_ok(out[:, pick], av, R.values(b[pick], sb[pick], fmt), 1.0, torch.float32, f"{fmt} {m} {n} {k}")
+    _product_ok(out[:, -1:], av, R.values(b[-1:], sb[-1:], fmt), 1.0, torch.float32, "last weight row")
+
+
+def test_experts_matmul_weights_past_32_bits(gpu_available):
+    """512 experts whose weights take 8 GB: the last ones' rows."""
+    m = pkg()
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB of free device memory")
+    n, k = 1 << 16, 256
+    b = torch.zeros(512, n, k, dtype=torch.uint8, device=DEV)
+    sb = torch.full((512, n, k // 32), 127, dtype=torch.uint8, device=DEV)
+    g = _gen(51)
+    w, sw = R.random_packed(g, (2,), 300, k, "mxfp8")
+    b[510:, -300:], sb[510:, -300:] = w.view(torch.uint8).to(DEV), sw.view(torch.uint8).to(DEV)
+    a, sa = R.random_packed(g, (), 20, k, "mxfp8")
+    off = torch.tensor([0] * 510 + [2, 3, 20], dtype=torch.int32, device=DEV)
+    out = m.experts_matmul_mx(a.to(DEV), sa.to(DEV), b.view(torch.float8_e4m3fn), sb.view(torch.float8_e8m0fnu), off,
+                              "mxfp8", out_dtype=torch.float32)
+    assert m.device_status() == 0 and (out[:, :-300] == 0).all() and (out[:2] == 0).all()
+    av = R.values(a, sa, "mxfp8")
+    _product_ok(out[2:3, -300:], av[2:3], R.values(w[0], sw[0], "mxfp8"), 1.0, torch.float32)
+    _product_ok(out[3:, -300:], av[3:], R.values(w[1], sw[1], "mxfp8"), 1.0, torch.float32)
+
+
+def test_products_of_the_most_rows(gpu_available):
+    """2^24 rows: their number of tiles, and outputs past 2^31 elements."""
+    m = pkg()
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB of free device memory")
+    rows, n, k = 1 << 24, 192, 32
+    g = _gen(52)
+    a, sa = R.random_packed(g, (), 1000, k, "mxfp4")
+    b, sb = R.random_packed(g, (2,), n, k, "mxfp4")
+    big = torch.zeros(rows, k // 2, dtype=torch.uint8, device=DEV)
+    sbig = torch.full((rows, 1), 127, dtype=torch.uint8, device=DEV)
+    big[-1000:], sbig[-1000:] = a.to(DEV), sa.view(torch.uint8).to(DEV)
+    sbig = sbig.view(torch.float8_e8m0fnu)
+    out = torch.full((rows, n), 5.0, dtype=torch.bfloat16, device=DEV)
+    m.matmul_mx(big, sbig, b[0].to(DEV), sb[0].to(DEV), "mxfp4", out=out)
+    assert m.device_status() == 0 and not out[:-1000].any()
+    av, bv = R.values(a, sa, "mxfp4"), R.values(b, sb, "mxfp4")
+    _product_ok(out[-1000:], av, bv[0], 1.0, torch.bfloat16)
+    out.fill_(5.0)
+    off = torch.tensor([7, rows - 500, rows - 1], dtype=torch.int32, device=DEV)
+    m.experts_matmul_mx(big, sbig, b.to(DEV), sb.to(DEV), off, "mxfp4", out=out)
+    assert m.device_status() == 0 and (out[:7] == 5).all() and (out[-1] == 5).all() and not out[7:-1000].any()
+    _product_ok(out[-1000:-500], av[:500], bv[0], 1.0, torch.bfloat16)
+    _product_ok(out[-500:-1], av[500:-1], bv[1], 1.0, torch.bfloat16)
+
+
 def test_products_are_repeatable_on_streams_and_in_graphs(gpu_available):
     """The same bits again, from two streams at once and from a replayed graph
     whose inputs have changed."""
