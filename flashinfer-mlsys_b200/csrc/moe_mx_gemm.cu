@@ -33,7 +33,7 @@
 //     without any loads (87 us), where its four MMAs are 512: the twelve scale
 //     copies and the issue of both do not hide behind them
 //   8192 x 7168 x 4096 mxfp8    174 us, 2.8 PFLOP/s: the card's power limit
-//   32 experts x 7168 x 4096 nvfp4, 64 rows   74 us, 6.0 TB/s: HBM
+//   32 experts x 7168 x 4096 nvfp4, 64 rows   71 us, 6.3 TB/s: HBM
 //   32 experts x 2048 x 7168 mxfp4, 8192 rows 88 us, 4.3 TB/s: eight stages a
 //     tile, in which neither HBM (55%) nor the tensor pipe (34%) is kept busy
 //   8 x 7168 x 4096 nvfp4       7.2 us: launch, one exchange across the
@@ -711,29 +711,67 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
           return mx_sf_shift(w[g][q], i, static_cast<int>((reinterpret_cast<uint64_t>(b) + r * ld + at) & 3u), left);
         }
       };
-      uint32_t w[1 + Cfg::kChunks][4][kR];
       uint32_t grp = 0;
-      for (int u = u_first; u < units && !mx_aborted(ctl); u += u_step) {
-        const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
-        bool ok = true;
-        for (int k = k0; k < k1; k += 4, ++grp) {
-          load(x, k, w);  // under way while the slot is still being read
-          const uint32_t gs = grp % Cfg::kGroups;
-          ok = all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp / Cfg::kGroups) & 1u) ^ 1u, kMxWaitNs));
-          if (!ok) break;
-          uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
-#pragma unroll
-          for (int i = 0; i < kW; ++i) {
-#pragma unroll
-            for (int g = 0; g <= Cfg::kChunks; ++g)
-              *reinterpret_cast<uint4*>(sf + (g == 0 ? i : kW + i * Cfg::kChunks + g - 1) * 512) =
-                  make_uint4(word(x, k, w, g, 0, i), word(x, k, w, g, 1, i), word(x, k, w, g, 2, i), word(x, k, w, g, 3, i));
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->sf_full[gs]);
+      // words of stages k .. k + 3 into the next slot
+      const auto put = [&](const MxUnit& x, int k, const uint32_t (&w)[1 + Cfg::kChunks][4][kR]) {
+        const uint32_t gs = grp % Cfg::kGroups;
+        if (!all_lanes(mbar_wait_bounded(&ctl->sf_empty[gs], ((grp / Cfg::kGroups) & 1u) ^ 1u, kMxWaitNs))) {
+          mx_abort(ctl);
+          return false;
         }
-        if (!ok) { mx_abort(ctl); break; }
+        uint8_t* sf = sfs + gs * Cfg::kGroupBytes + j * Cfg::kSfBytes + r0 * 16;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+#pragma unroll
+          for (int g = 0; g <= Cfg::kChunks; ++g)
+            *reinterpret_cast<uint4*>(sf + (g == 0 ? i : kW + i * Cfg::kChunks + g - 1) * 512) =
+                make_uint4(word(x, k, w, g, 0, i), word(x, k, w, g, 1, i), word(x, k, w, g, 2, i), word(x, k, w, g, 3, i));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->sf_full[gs]);
+        ++grp;
+        return true;
+      };
+      if (kPair || clustered) {
+        uint32_t w[1 + Cfg::kChunks][4][kR];
+        bool ok = true;
+        for (int u = u_first; u < units && ok && !mx_aborted(ctl); u += u_step) {
+          const MxUnit x = mx_unit(ctl, p, u, ntn, kTileRows);
+          for (int k = k0; k < k1 && ok; k += 4) {
+            load(x, k, w);  // under way while the slot is still being read
+            ok = put(x, k, w);
+          }
+        }
+      } else if (u_first < units) {
+        // A CTA by itself streams weights, whose scales come from HBM: the next
+        // group's loads start before this one's are waited for. 32 experts x
+        // 7168 x 4096 nvfp4, 64 rows on 27 of them: 74.2 -> 70.9 us. (A split has a group or
+        // two and loses 4% to the longer code; in a pair both groups' words do
+        // not fit the registers, and a group takes longer to use than to load.)
+        MxUnit xa = mx_unit(ctl, p, u_first, ntn, kTileRows), xb = xa;
+        int u = u_first, ka = k0, kb = k0;
+        uint32_t wa[1 + Cfg::kChunks][4][kR], wb[1 + Cfg::kChunks][4][kR];
+        // the group behind (x, k): false where there is none
+        const auto next = [&](const MxUnit& x, int k, MxUnit& y, int& l) {
+          y = x;
+          l = k + 4;
+          if (l < k1) return true;
+          l = k0;
+          u += u_step;
+          if (u >= units || mx_aborted(ctl)) return false;
+          y = mx_unit(ctl, p, u, ntn, kTileRows);
+          return true;
+        };
+        load(xa, ka, wa);
+        while (true) {
+          bool more = next(xa, ka, xb, kb);
+          if (more) load(xb, kb, wb);
+          if (!put(xa, ka, wa) || !more) break;
+          more = next(xb, kb, xa, ka);
+          if (more) load(xa, ka, wa);
+          if (!put(xb, kb, wb) || !more) break;
+        }
       }
     };
     if (kW == 4 && (low & 15) == 0)
