@@ -33,9 +33,11 @@
 //     without any loads (87 us), where its four MMAs are 512: the twelve scale
 //     copies and the issue of both do not hide behind them
 //   8192 x 7168 x 4096 mxfp8    174 us, 2.8 PFLOP/s: the card's power limit
-//   32 experts x 7168 x 4096 nvfp4, 64 rows   71 us, 6.3 TB/s: HBM
-//   32 experts x 2048 x 7168 mxfp4, 8192 rows 88 us, 4.3 TB/s: eight stages a
-//     tile, in which neither HBM (55%) nor the tensor pipe (34%) is kept busy
+//   32 experts x 7168 x 4096 nvfp4, 64 rows   71 us, 6.3 TB/s: HBM (27 experts
+//     with rows; 28 are 79 us, as their tiles are 6.05 waves of CTAs)
+//   32 experts x 2048 x 7168 mxfp4, 8192 rows 87 us, 4.3 TB/s: eight stages a
+//     tile, in which neither HBM (55%) nor the tensor pipe (34%) is kept busy;
+//     the MMA issuer waits in turn for tiles, scales and accumulators
 //   8 x 7168 x 4096 nvfp4       7.2 us: launch, one exchange across the
 //     cluster and some 2.6 us of weights
 #include <atomic>
