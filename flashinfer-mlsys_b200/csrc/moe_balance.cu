@@ -135,13 +135,15 @@ __device__ __forceinline__ int bal_first(const BalArgs& a, int64_t t) {
 
 // The logits of rows t, t + kBalWarps, ... (nb of them, at most kB) -> scores
 // a_j (0 in columns that are not there); rz: 1 / their sum, 0 where the scores
-// sum to zero. The exponential's and the quotient's fast forms: within 4 + 1.2
-// |l| steps of float32 together (scores of -80 then are 1e-5 off and weigh
-// nothing), a third of the operations, which bound these kernels: 65536 x 256
-// fp32 forward and backward 54.9 -> 47.8 us.
-template <int kDt, int kV, int kJ, int kB>
-__device__ __forceinline__ void bal_scores(const BalArgs& a, int64_t t, int nb, int lane, float (&x)[kB][kJ * kV],
-                                           float (&rz)[kB]) {
+// sum to zero. For the gradient (kBack) x becomes d a_j / d l_j instead, a
+// sigmoid's y (1 - y) as y e y with e = exp(-l), as 1 - y has lost all digits of
+// a y near 1; and dot becomes sum_j f_j a_j. The exponential's and the
+// quotient's fast forms: within 4 + 1.2 |l| steps of float32 together (scores of
+// -80 then are 1e-5 off and weigh nothing), a third of the operations, which
+// bound these kernels: 65536 x 256 fp32 forward and backward 54.9 -> 47.8 us.
+template <int kDt, int kV, int kJ, int kB, bool kBack>
+__device__ __forceinline__ void bal_scores(const BalArgs& a, int64_t t, int nb, int lane, const float* f,
+                                           float (&x)[kB][kJ * kV], float (&rz)[kB], float (&dot)[kB]) {
   constexpr int kSize = kDt == 2 ? 4 : 2;
 #pragma unroll
   for (int b = 0; b < kB; ++b) {
@@ -172,20 +174,34 @@ __device__ __forceinline__ void bal_scores(const BalArgs& a, int64_t t, int nb, 
 #pragma unroll
   for (int b = 0; b < kB; ++b) {
     rz[b] = 0.f;
+    dot[b] = 0.f;
     if (b >= nb) continue;
     if (a.softmax) {
       // a row of -inf: exp(-inf - 0) = 0 everywhere (a NaN row keeps its NaN)
       const float top = m[b] == -INFINITY ? 0.f : m[b];
 #pragma unroll
-      for (int i = 0; i < kJ * kV; ++i) x[b][i] = __expf(x[b][i] - top);
+      for (int i = 0; i < kJ * kV; ++i) {
+        const float y = __expf(x[b][i] - top);
+        rz[b] += y;
+        if constexpr (kBack) dot[b] = fmaf(f[i], y, dot[b]);
+        x[b][i] = y;
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < kJ * kV; ++i) x[b][i] = __fdividef(1.0f, 1.0f + __expf(-x[b][i]));
+      for (int i = 0; i < kJ * kV; ++i) {
+        const float e = __expf(-x[b][i]), y = __fdividef(1.0f, 1.0f + e);  // 0 where e passes 2^126
+        rz[b] += y;
+        if constexpr (kBack) {
+          dot[b] = fmaf(f[i], y, dot[b]);
+          x[b][i] = fminf(e, 0x1p127f) * y * y;
+        } else {
+          x[b][i] = y;
+        }
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kJ * kV; ++i) rz[b] += x[b][i];
   }
   warp_sums(rz);
+  if constexpr (kBack) warp_sums(dot);
 #pragma unroll
   for (int b = 0; b < kB; ++b) rz[b] = rz[b] == 0.f ? 0.f : 1.0f / rz[b];
 }
@@ -227,9 +243,9 @@ __global__ void __launch_bounds__(kBalThreads, kJ * kV <= 8 ? 2 : 1)
     for (int i = 0; i < kJ * kV; ++i) acc[i] = 0.f;
     constexpr int kB = bal_batch(kJ * kV);
     for (int64_t t = lo + warp; t < hi; t += kB * kBalWarps) {
-      float x[kB][kJ * kV], rz[kB];
+      float x[kB][kJ * kV], rz[kB], unused[kB];
       const int nb = bal_rows<kB>(t, hi);
-      bal_scores<kDt, kV, kJ, kB>(a, t, nb, lane, x, rz);
+      bal_scores<kDt, kV, kJ, kB, false>(a, t, nb, lane, nullptr, x, rz, unused);
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         if (b >= nb) break;
@@ -347,7 +363,7 @@ __global__ void __launch_bounds__(kBalThreads, kJ * kV <= 8 ? 2 : 1)
     hi = hi < t1 ? hi : t1;
     if (lo >= hi) continue;
     zero(done, lo);
-    const float unit = static_cast<float>(a.E) / (static_cast<float>(a.K) * len);
+    const float per = static_cast<float>(a.E) / (static_cast<float>(a.K) * len);  // f of one slot
     const float g = grad_loss[s] * a.coeff / len;
     float f[kJ * kV];
 #pragma unroll
@@ -355,21 +371,13 @@ __global__ void __launch_bounds__(kBalThreads, kJ * kV <= 8 ? 2 : 1)
 #pragma unroll
       for (int v = 0; v < kV; ++v) {
         const int c = (j * 32 + lane) * kV + v;
-        f[j * kV + v] = c < a.E ? unit * static_cast<float>(counts[static_cast<int64_t>(s) * a.E + c]) : 0.f;
+        f[j * kV + v] = c < a.E ? per * static_cast<float>(counts[static_cast<int64_t>(s) * a.E + c]) : 0.f;
       }
     constexpr int kB = bal_batch(kJ * kV);
     for (int64_t t = lo + warp; t < hi; t += kB * kBalWarps) {
       float x[kB][kJ * kV], rz[kB], dot[kB];
       const int nb = bal_rows<kB>(t, hi);
-      bal_scores<kDt, kV, kJ, kB>(a, t, nb, lane, x, rz);
-#pragma unroll
-      for (int b = 0; b < kB; ++b) {
-        dot[b] = 0.f;
-        if (b >= nb) continue;
-#pragma unroll
-        for (int i = 0; i < kJ * kV; ++i) dot[b] = fmaf(f[i], x[b][i], dot[b]);
-      }
-      warp_sums(dot);
+      bal_scores<kDt, kV, kJ, kB, true>(a, t, nb, lane, f, x, rz, dot);
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         if (b >= nb) break;
@@ -381,11 +389,7 @@ __global__ void __launch_bounds__(kBalThreads, kJ * kV <= 8 ? 2 : 1)
           const int c = (j * 32 + lane) * kV;
           float d[kV];
 #pragma unroll
-          for (int v = 0; v < kV; ++v) {
-            const float y = x[b][j * kV + v];
-            d[v] = g * (y * rz[b]) * (f[j * kV + v] - mean);
-            if (!a.softmax) d[v] *= 1.0f - y;
-          }
+          for (int v = 0; v < kV; ++v) d[v] = g * (x[b][j * kV + v] * rz[b]) * (f[j * kV + v] - mean);
           if (c < a.E) bal_store<kDt, kV>(row, c, d);
         }
       }

@@ -231,3 +231,85 @@ def test_refusals(gpu_available):
                  lambda: m.balance_loss(x, ids, torch.zeros(1, dtype=torch.int32, device=DEV))):
         with pytest.raises(ValueError):
             call()
+
+
+def _formula(x, ids, off, grad, score, coeff):
+    """The gradient from its formula in float64, and the sum of its two terms'
+    sizes. The sigmoid's complement is sigmoid(-l), which no difference cancels."""
+    x = x.double()
+    (T, E), K = x.shape, ids.shape[1]
+    ref, size = torch.zeros(T, E, dtype=torch.float64), torch.zeros(T, E, dtype=torch.float64)
+    for s, (lo, hi) in enumerate(zip(off[:-1].tolist(), off[1:].tolist())):
+        if hi <= lo:
+            continue
+        r = x[lo:hi]
+        p = torch.softmax(r, 1) if score == "softmax" else r.sigmoid() / r.sigmoid().sum(1, keepdim=True)
+        f = torch.bincount(ids[lo:hi].flatten().long(), minlength=E).double() * E / (K * (hi - lo))
+        unit = grad[s].double() * coeff / (hi - lo) * p * (1.0 if score == "softmax" else (-r).sigmoid())
+        mean = (p * f).sum(1, keepdim=True)
+        ref[lo:hi], size[lo:hi] = unit * (f - mean), unit * (f + mean)
+    return ref, size
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("low,high", [(8, 16), (10, 40), (17, 30), (-40, 40), (-80, -20)])
+@pytest.mark.parametrize("T,E,K,S", [(40, 16, 2, 3), (33, 60, 4, 2), (70, 256, 8, 4), (20, 1024, 8, 2), (12, 513, 6, 2)])
+def test_gradient_of_large_logits(gpu_available, T, E, K, S, low, high, dtype):
+    """The sigmoid's factor 1 - sigmoid(l) is e^-16 and less here: the error
+    stays relative to the gradient's own terms, this factor included."""
+    _, ids, off, grad = _inputs(T, E, K, S, torch.float32, T + E)
+    x = (low + (high - low) * torch.rand(T, E, generator=torch.Generator().manual_seed(E))).to(R.DTYPES[dtype])
+    xd = x.to(DEV).requires_grad_(True)
+    loss, _ = pkg().balance_loss(xd, ids.to(DEV), off.to(DEV), 0.3)
+    dx, = torch.autograd.grad(loss, xd, grad.to(DEV))
+    ref, size = _formula(x, ids, off, grad, "sigmoid", 0.3)
+    # as in _check, and for the factor an exponential, a sum, a quotient and two products: 16 half-steps more
+    rel = (144 + E / 32 + T / 64) * 2.0 ** -24
+    tol = rel * size + torch.finfo(x.dtype).eps / 2 * 1.01 * ref.abs() + torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps
+    assert ((dx.cpu().double() - ref).abs() <= tol).all()
+
+
+def test_gradient_of_saturated_rows_against_differences(gpu_available):
+    """Rows whose float32 sigmoids are all 1: differences of the loss in
+    float64, p_j = (1 - c_j) / sum (1 - c) with c = sigmoid(-l)."""
+    T, E = 4, 8
+    g = torch.Generator().manual_seed(3)
+    x = 12 + 8 * torch.rand(T, E, generator=g)
+    x[1] += 6
+    ids = torch.tensor([[0, 1], [2, 0], [0, 3], [1, 0]], dtype=torch.int32)
+    xd = x.to(DEV).requires_grad_(True)
+    loss, _ = pkg().balance_loss(xd, ids.to(DEV), None, 1.0)
+    dx, = torch.autograd.grad(loss.sum(), xd)
+    f = torch.bincount(ids.flatten().long(), minlength=E).double() * E / (2 * T)
+
+    def change(t, j, d):
+        """loss(l_tj + d) - loss(l_tj) without a difference of nearly equal numbers: the change of a_j is
+        D = c (1 - e^-d) / (1 + e^(-l-d)), and that of sum_i f_i p_i is D (f_j - mean) / (sum + D)."""
+        a = x[t].double().sigmoid()
+        c = (-x[t, j].double()).sigmoid()
+        dj = -c * torch.expm1(torch.tensor(-d, dtype=torch.float64)) / (1 + torch.exp(-x[t, j].double() - d))
+        mean = (f * a).sum() / a.sum()
+        return dj * (f[j] - mean) / (a.sum() + dj) / T
+
+    for t in range(T):
+        for j in range(E):
+            # the gradient is u (f_j - mean), u = c / (T sum): its error is (144 + ..) 2^-24 < 2^-16 of u (f_j + mean),
+            # whatever the difference leaves (f_2 = 1 and mean is 1 + 1e-6 here); the odd terms of the central
+            # difference add h^2 / 6 of it
+            d = float(change(t, j, 1e-4) - change(t, j, -1e-4)) / 2e-4
+            a = x[t].double().sigmoid()
+            u = float((-x[t, j].double()).sigmoid() / a.sum() / T)
+            assert abs(d - float(dx[t, j])) <= 2.0 ** -16 * u * float(f[j] + (f * a).sum() / a.sum())
+
+
+def test_gradient_of_tiny_scores_under_a_large_factor(gpu_available):
+    """Scores near 2^-126, whose sum's reciprocal is near 2^126, and a loss that is scaled by 10^6."""
+    x = -86.5 + torch.rand(8, 4, generator=torch.Generator().manual_seed(1))
+    ids = torch.arange(8, dtype=torch.int32).remainder(3)[:, None]
+    grad = torch.tensor([1e6])
+    xd = x.to(DEV).requires_grad_(True)
+    loss, _ = pkg().balance_loss(xd, ids.to(DEV), None, 1.0)
+    dx, = torch.autograd.grad(loss, xd, grad.to(DEV))
+    ref, size = _formula(x, ids, torch.tensor([0, 8]), grad, "sigmoid", 1.0)
+    # the exponential's bound is relative to |l|: 2 |l| half-steps above those of test_gradient_of_large_logits
+    assert ((dx.cpu().double() - ref).abs() <= (144 + 4 * 87) * 2.0 ** -24 * size).all()
