@@ -311,5 +311,23 @@ def test_gradient_of_tiny_scores_under_a_large_factor(gpu_available):
     loss, _ = pkg().balance_loss(xd, ids.to(DEV), None, 1.0)
     dx, = torch.autograd.grad(loss, xd, grad.to(DEV))
     ref, size = _formula(x, ids, torch.tensor([0, 8]), grad, "sigmoid", 1.0)
-    # the exponential's bound is relative to |l|: 2 |l| half-steps above those of test_gradient_of_large_logits
-    assert ((dx.cpu().double() - ref).abs() <= (144 + 4 * 87) * 2.0 ** -24 * size).all()
+    assert ((dx.cpu().double() - ref).abs() <= 144 * 2.0 ** -24 * size).all()  # as in test_gradient_of_large_logits
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E", [8, 256])
+def test_small_scores_keep_their_precision(gpu_available, score, E):
+    """Sequences of one token whose slots all name an expert with a score of
+    e^-20 to e^-80: the loss is that score's share, one value each. Logits are
+    multiples of 1/8, so that their differences are exact."""
+    T = 200
+    g = torch.Generator().manual_seed(E)
+    x = torch.randint(-8, 9, (T, E), generator=g).float() / 8
+    x[:, 3] = -torch.randint(160, 640, (T,), generator=g).float() / 8
+    ids = torch.full((T, 1), 3, dtype=torch.int32)
+    loss, _ = pkg().balance_loss(x.to(DEV), ids.to(DEV), torch.arange(T + 1, dtype=torch.int32, device=DEV), 1.0, score)
+    a = x.double().sigmoid() if score == "sigmoid" else torch.softmax(x.double(), 1)
+    want = E * (a / a.sum(1, keepdim=True))[:, 3]
+    # half-steps of 2^-24: an exponential 4, sum 1, quotient 4, product 1, of numerator and sum; the sum's E / 32
+    # + 5 additions; its reciprocal and the product 2; the store 1
+    assert ((loss.cpu().double() - want).abs() <= (28 + E / 32) * 2.0 ** -24 * want).all()
