@@ -7,6 +7,7 @@ runs in ``libmoe_fp8_ds.so`` on the current CUDA stream; there is no fallback.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .mx import _bad, _cuda, _run
@@ -67,7 +68,8 @@ def balance_loss(routing_logits: torch.Tensor, topk_ids: torch.Tensor, seq_offse
     score(l_tj)`` and ``loss[s] = coeff * sum_i f_i * mean_t p_ti``.
 
     * routing_logits: [T, E] float32, bf16 or fp16 (E <= 1024, rows any stride
-      apart); the loss is differentiable with respect to it, f is constant
+      apart); the loss can be differentiated with respect to it once, in reverse
+      mode (another derivative raises ``RuntimeError``); f is constant
     * topk_ids: int32 [T, K] (``route``'s ids). Ids outside [0, E) are not
       counted, an id that occurs twice counts twice
     * seq_offsets: int32 [S + 1] on the device, not decreasing: sequence s is
@@ -110,6 +112,8 @@ def balance_loss(routing_logits: torch.Tensor, topk_ids: torch.Tensor, seq_offse
             _bad(f"seq_offsets must be on {dev}")
         if not seq_offsets.is_contiguous():
             _bad("seq_offsets must be contiguous")
+    if forward_ad.unpack_dual(routing_logits).tangent is not None:
+        raise RuntimeError("balance_loss has no forward-mode derivative")
     if routing_logits.requires_grad and torch.is_grad_enabled():
         return _BalanceLoss.apply(routing_logits, topk_ids, seq_offsets, float(coeff), score)
     return _forward(routing_logits, topk_ids, seq_offsets, float(coeff), score)

@@ -331,3 +331,19 @@ def test_small_scores_keep_their_precision(gpu_available, score, E):
     # half-steps of 2^-24: an exponential 4, sum 1, quotient 4, product 1, of numerator and sum; the sum's E / 32
     # + 5 additions; its reciprocal and the product 2; the store 1
     assert ((loss.cpu().double() - want).abs() <= (28 + E / 32) * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(gpu_available, requires_grad):
+    """A dual tensor's tangent is not dropped: the call says that it has no forward-mode derivative."""
+    x, ids, off, _ = _inputs(8, 16, 2, 1, torch.float32, 9)
+    xd = x.to(DEV).requires_grad_(requires_grad)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        dual = fw.make_dual(xd, torch.ones_like(xd))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            pkg().balance_loss(dual, ids.to(DEV), off.to(DEV))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            pkg().balance_loss(dual, ids.to(DEV), off.to(DEV))
+        loss, _ = pkg().balance_loss(xd, ids.to(DEV), off.to(DEV))  # no tangent: as ever
+    assert torch.equal(loss, pkg().balance_loss(xd, ids.to(DEV), off.to(DEV))[0])
