@@ -77,12 +77,13 @@ __device__ __forceinline__ uint32_t mx_block_max(uint32_t m) {
 }
 
 // RN(x / d) by Markstein's correction (P. Markstein, IA-64 division, 1990):
-// with r = RN(1/d) and q0 = RN(x r), the remainder x - q0 d is exact in one
-// fma and RN(q0 + remainder r) is the correctly rounded quotient while nothing
-// leaves the normal range.
+// with r = RN(1/d) and q0 = RN(x r), the remainder q0 d - x is exact in one
+// fma and RN(q0 - remainder r) is the correctly rounded quotient while nothing
+// leaves the normal range. (The remainder's sign matters for x = -0: of q0 = -0
+// only a subtraction of +0 keeps the sign.)
 __device__ __forceinline__ float mx_quotient(float x, float d, float r) {
   const float q0 = x * r;
-  return fmaf(fmaf(-q0, d, x), r, q0);
+  return fmaf(-fmaf(q0, d, -x), r, q0);
 }
 __device__ __forceinline__ bool mx_mid(float v) { return v > 0x1p-60f && v < 0x1p60f; }
 

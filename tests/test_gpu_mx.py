@@ -545,3 +545,20 @@ def test_expert_mlp_after_routing(gpu_available, fmt):
         _product_ok(h[r], av[r], R.values(w13[e].cpu(), s13[e].cpu(), fmt), 1.0, torch.float32)
         _product_ok(y[r], iv[r], R.values(w2[e].cpu(), s2[e].cpu(), fmt), 1.0, torch.float32)
     assert out.isfinite().all() and (out.abs().sum(1) > 0).any()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("g", [None, 0.37, 1e-30])
+def test_quantize_keeps_the_sign_of_zero(gpu_available, fmt, dtype, g):
+    """x / s is -0 where x is: single -0 among ordinary values, in every branch of the scale."""
+    x = _hidden(11, 256, R.DTYPES[dtype], 21)
+    x[torch.rand(11, 256, generator=_gen(22)) < 0.2] = -0.0
+    x[5] = 1.0
+    x[5, ::3] = -0.0
+    gs = torch.tensor([g]) if g and fmt == "nvfp4" else None
+    q, s = pkg().quantize_mx(x.to(DEV), fmt, None if gs is None else gs.to(DEV))
+    _quantised(fmt, q, s, x, gs)
+    if gs is None:
+        q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, None, fmt=fmt)
+        _quantised(fmt, q, s, x)
