@@ -4,7 +4,7 @@
 // All three are one pass over the data and HBM-bound. The register bounds are
 // measured at 16384 x 7168: 16-bit rows gain 3 to 5% from more CTAs on an SM
 // (the norm 149 -> 142 us with nvfp4, 140 -> 136 us with mxfp8), fp32 rows
-// would spill (233 -> 354 us). At 16384 x 7168 bf16: quantisation 54 us nvfp4
+// would spill (233 -> 354 us) and keep three CTAs (two: 140 us at 8192 rows, not 119). At 16384 x 7168 bf16: quantisation 54 us nvfp4
 // (5.5 TB/s; some 12 instructions a value nearly bind), 46 us mxfp4, 52 us mxfp8
 // (6.8 TB/s), dequantisation 45 us (6.6 TB/s), residual + norm + mxfp8 136 us
 // (6.1 TB/s); fp32 rows 6.3 to 7.1 TB/s.
@@ -138,22 +138,54 @@ __global__ void __launch_bounds__(kMxThreads)
   }
 }
 
-// h * w / sqrt(v), rounded to odd: cut off to float32, with the last bit set
-// where something was cut. A second rounding, to a format of at most 22 bits,
-// then gives what rounding the exact value would, so the quantisation that
-// follows sees no float32 tie that is none. inv = hi + lo is 1 / sqrt(v) to some
-// 2^-48; h w is exact as p (16-bit types) or p + e. `cut`: lo is not zero, so
-// that no product is a float32; rows with lo = 0 (1 / sqrt(v) is a float32)
-// look at the remainder.
+// Two floats at a time: the same operations in half the instructions.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma_rz(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Two values h * w / sqrt(v), rounded to odd: cut off to float32, with the last
+// bit set where something was cut. A second rounding, to a format of at most 22
+// bits, then gives what rounding the exact value would, so the quantisation that
+// follows sees no float32 tie that is none. 1 / sqrt(v) lies between hi + lo0
+// and hi + lo1; h w is exact as p (16-bit types) or p + e. Where the bounds cut
+// to two float32 numbers, the value is the outer one to within the bounds and
+// is taken for it: a row of +-7 has y = +-1, not the number below. One value at a
+// time the second bound costs 3% (16384 x 7168 bf16 mxfp8: 140 us, in pairs 136 us).
 template <int kDt>
-__device__ __forceinline__ float mx_norm_value(float h, float w, float hi, float lo, bool cut) {
-  const float p = __fmul_rn(h, w);
-  float t = __fmul_rn(p, lo);
-  if (kDt == kDtFp32) t = fmaf(fmaf(h, w, -p), hi, t);
-  const float y = __fmaf_rz(p, hi, t);
-  if (cut) return __uint_as_float(__float_as_uint(y) | 1u);
-  const bool rest = fmaf(p, hi, -y) != -t;
-  return __uint_as_float(__float_as_uint(y) | (rest ? 1u : 0u));
+__device__ __forceinline__ void mx_norm_pair(float* h, const float* w, uint64_t hi, uint64_t lo0, uint64_t lo1) {
+  const uint64_t h2 = f2_pack(h[0], h[1]), w2 = f2_pack(w[0], w[1]);
+  const uint64_t p = f2_mul(h2, w2);
+  uint64_t t0 = f2_mul(p, lo0), t1 = f2_mul(p, lo1);
+  if (kDt == kDtFp32) {
+    const uint64_t e = f2_fma(h2, w2, p ^ 0x8000000080000000ull);
+    t0 = f2_fma(e, hi, t0);
+    t1 = f2_fma(e, hi, t1);
+  }
+  float in[2], out[2];
+  f2_unpack(f2_fma_rz(p, hi, t0), in, in + 1);
+  f2_unpack(f2_fma_rz(p, hi, t1), out, out + 1);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) h[i] = __uint_as_float(__float_as_uint(out[i]) | (in[i] == out[i] ? 1u : 0u));
 }
 
 constexpr int kNormPer = 2;  // spans of a thread
@@ -166,7 +198,7 @@ constexpr int kNormPer = 2;  // spans of a thread
 // decides how often a value lands on the wrong side of a border of the format.
 // Without a weight: y = h.
 template <int kFmt, int kDt, int kMaxT>
-__global__ void __launch_bounds__(kMaxT, kMaxT == 256 && kDt != kDtFp32 ? 5 : 1)
+__global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3) : 1)
     mx_norm_kernel(const uint8_t* __restrict__ x, int64_t x_ld_bytes, uint8_t* residual, int64_t res_ld_bytes,
                    const uint8_t* __restrict__ weight, bool wide, float eps, int64_t rows, uint32_t per_row,
                    uint32_t tpr, const float* __restrict__ global_scale, uint8_t* __restrict__ q,
@@ -211,21 +243,17 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 && kDt != kDtFp32 ? 5 : 1)
       mx_store<kW>(rp + static_cast<int64_t>(j) * tpr * kB, wide, w[j]);
     }
   }
-  float hi = 1.f, lo = 0.f;
+  float hi = 1.f, lo0 = 0.f, lo1 = 0.f;
   if (weight) {
-    double ss = 0.0;
+    double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
     for (int j = 0; j < kNormPer; ++j) {
       float f[kMxSpan];
       mx_to_float<kDt>(w[j], f);
 #pragma unroll
-      for (int i = 0; i < kMxSpan; i += 8) {
-        float a[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = fmaf(f[i + 2 * k + 1], f[i + 2 * k + 1], f[i + 2 * k] * f[i + 2 * k]);
-        ss += static_cast<double>((a[0] + a[1]) + (a[2] + a[3]));
-      }
+      for (int i = 0; i < kMxSpan; ++i) part[i % 4] = fma(static_cast<double>(f[i]), static_cast<double>(f[i]), part[i % 4]);
     }
+    double ss = (part[0] + part[1]) + (part[2] + part[3]);
     for (uint32_t off = whole ? 16 : tpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     if (whole) {
       if ((tid & 31) == 0) warp_ss[tid >> 5] = ss;
@@ -234,20 +262,25 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 && kDt != kDtFp32 ? 5 : 1)
       for (uint32_t i = 0; i < blockDim.x / 32; ++i) ss += warp_ss[i];
     }
     const double v = ss / static_cast<double>(per_row * kMxSpan) + static_cast<double>(eps);
-    // 1 / sqrt(v): one Newton step from the float32 estimate (2^-22) where that
-    // is an ordinary number, else the plain operations (zero rows, huge ones)
+    // 1 / sqrt(v): two Newton steps from the float32 estimate (2^-22, 2^-43,
+    // 2^-51) where that is an ordinary number, else the plain operations (zero
+    // rows, huge ones)
     double inv;
     if (v > 1e-30 && v < 1e30) {
-      const double r = static_cast<double>(rsqrtf(static_cast<float>(v)));
-      inv = fma(r * fma(-v * r, r, 1.0), 0.5, r);
+      inv = static_cast<double>(rsqrtf(static_cast<float>(v)));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) inv = fma(inv * fma(-v * inv, inv, 1.0), 0.5, inv);
     } else {
       inv = 1.0 / sqrt(v);
     }
     hi = static_cast<float>(inv);
-    lo = static_cast<float>(inv - static_cast<double>(hi));
-    if (!(fabsf(hi) < INFINITY)) lo = 0.f;
+    if (fabsf(hi) < INFINITY) {
+      // the sum is within 2^-47, its root's reciprocal within 2^-48; lo and its products add 2^-47
+      const float lo = static_cast<float>(inv - static_cast<double>(hi));
+      lo0 = lo - 0x1p-42f * hi;
+      lo1 = lo + 0x1p-42f * hi;
+    }
   }
-  const bool cut = lo != 0.f;
   const MxGlobal gl = mx_global(kFmt == kFmtNvfp4 ? global_scale : nullptr);
 #pragma unroll
   for (int j = 0; j < kNormPer; ++j) {
@@ -268,7 +301,8 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 && kDt != kDtFp32 ? 5 : 1)
       float wf[kMxSpan];
       mx_to_float<kDt>(ww, wf);
 #pragma unroll
-      for (int i = 0; i < kMxSpan; ++i) f[i] = mx_norm_value<kDt>(f[i], wf[i], hi, lo, cut);
+      for (int i = 0; i < kMxSpan; i += 2)
+        mx_norm_pair<kDt>(f + i, wf + i, f2_pack(hi, hi), f2_pack(lo0, lo0), f2_pack(lo1, lo1));
     }
     const uint32_t am = mx_block_max<kFmt>(mx_span_max(f));
     uint32_t p[4];
@@ -319,7 +353,7 @@ cudaError_t norm_launch(const MxNormCall& c, cudaStream_t s) {
                     static_cast<const uint8_t*>(c.weight), wide, c.eps, c.rows, per_row, tpr, c.global_scale,
                     static_cast<uint8_t*>(c.q), static_cast<uint8_t*>(c.scale));
   };
-  // rows of up to 8192 columns keep a bound that leaves the compiler 255 registers
+  // rows of up to 8192 columns take the variants of 256 threads, with their bounds on registers
   if (threads <= 256) return go(mx_norm_kernel<kFmt, kDt, 256>);
   return go(mx_norm_kernel<kFmt, kDt, 1024>);
 }

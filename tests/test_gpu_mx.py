@@ -562,3 +562,33 @@ def test_quantize_keeps_the_sign_of_zero(gpu_available, fmt, dtype, g):
     if gs is None:
         q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, None, fmt=fmt)
         _quantised(fmt, q, s, x)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("cols", [32, 96, 512, 1024, 7168, 32768])
+def test_norm_of_exact_quotients(gpu_available, fmt, dtype, cols):
+    """Rows whose y is a short number although 1 / sqrt(v) is none: +-c alone,
+    one entry in four (y = 2 w), nine in sixteen (4/3 w), and c = 3, eps = 7 (3/4
+    w), with weights that put y on borders and ties of the formats. Codes and
+    scales are y's."""
+    dt = R.DTYPES[dtype]
+    g = _gen(cols)
+    w = torch.tensor([1.0, 0.75, 1.0625, 1.1875, 1.25, 3.5, 5.0, 0.25])[torch.randint(0, 8, (cols,), generator=g)]
+    w[:32] = 1.0
+    for c in (7.0, 13.0, 14.0, 49.0, 0.1, 1e-3, 517.0):
+        sign = torch.randint(0, 2, (6, cols), generator=g) * 2.0 - 1.0
+        part = sign.clone()
+        part.view(6, -1, 4)[:, :, 1:] = 0.0
+        for rows, scale in ((sign, 1.0), (part, 2.0)):
+            x = (rows * torch.tensor(c)).to(dt)
+            q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, w.to(dt).to(DEV), 0.0, fmt)
+            _quantised(fmt, q, s, rows * scale * w)
+        nine = sign.clone()
+        nine.view(6, -1, 16)[:, :, ::2] = 0.0
+        nine.view(6, -1, 16)[:, :, 8] = 1.0
+        q, s = pkg().add_rmsnorm_quantize_mx((nine * torch.tensor(c)).to(dt).to(DEV), None, (0.75 * w).to(dt).to(DEV), 0.0, fmt)
+        _quantised(fmt, q, s, nine * w)
+    x = (sign * 3.0).to(dt)
+    q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, w.to(dt).to(DEV), 7.0, fmt)
+    _quantised(fmt, q, s, sign * 0.75 * w)
