@@ -171,15 +171,16 @@ __device__ __forceinline__ uint64_t f2_fma_rz(uint64_t a, uint64_t b, uint64_t c
 // to two float32 numbers, the value is the outer one to within the bounds and
 // is taken for it: a row of +-7 has y = +-1, not the number below. One value at a
 // time the second bound costs 3% (16384 x 7168 bf16 mxfp8: 140 us, in pairs 136 us).
+constexpr uint64_t kMinus = 0x8000000080000000ull;  // both signs
 template <int kDt>
 __device__ __forceinline__ void mx_norm_pair(float* h, const float* w, uint64_t hi, uint64_t lo0, uint64_t lo1) {
   const uint64_t h2 = f2_pack(h[0], h[1]), w2 = f2_pack(w[0], w[1]);
   const uint64_t p = f2_mul(h2, w2);
   uint64_t t0 = f2_mul(p, lo0), t1 = f2_mul(p, lo1);
   if (kDt == kDtFp32) {
-    const uint64_t e = f2_fma(h2, w2, p ^ 0x8000000080000000ull);
-    t0 = f2_fma(e, hi, t0);
-    t1 = f2_fma(e, hi, t1);
+    const uint64_t e = f2_fma(h2 ^ kMinus, w2, p);  // -e, +0 of zeros: what is subtracted leaves a -0 as it is
+    t0 = f2_fma(e, hi ^ kMinus, t0);
+    t1 = f2_fma(e, hi ^ kMinus, t1);
   }
   float in[2], out[2];
   f2_unpack(f2_fma_rz(p, hi, t0), in, in + 1);
@@ -273,9 +274,10 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3)
     } else {
       inv = 1.0 / sqrt(v);
     }
-    hi = static_cast<float>(inv);
-    if (fabsf(hi) < INFINITY) {
-      // the sum is within 2^-47, its root's reciprocal within 2^-48; lo and its products add 2^-47
+    // the sum is within 2^-47, its root's reciprocal within 2^-48; lo and its products
+    // add 2^-46. Neither bound's lo is negative: the products of -0 stay -0
+    hi = __double2float_rd(inv * (1.0 - 0x1p-41));
+    if (hi < INFINITY) {
       const float lo = static_cast<float>(inv - static_cast<double>(hi));
       lo0 = lo - 0x1p-42f * hi;
       lo1 = lo + 0x1p-42f * hi;

@@ -592,3 +592,21 @@ def test_norm_of_exact_quotients(gpu_available, fmt, dtype, cols):
     x = (sign * 3.0).to(dt)
     q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, w.to(dt).to(DEV), 7.0, fmt)
     _quantised(fmt, q, s, sign * 0.75 * w)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows,cols", [(40, 64), (40, 1024)])
+def test_norm_keeps_the_sign_of_zero(gpu_available, fmt, dtype, rows, cols):
+    """y = h w / sqrt(v) is -0 where h is -0 and w is positive, or the other way round."""
+    g = _gen(80 + cols)
+    x = torch.randn(rows, cols, generator=g).to(R.DTYPES[dtype])
+    w = (torch.randint(0, 2, (cols,), generator=g) * 2.0 - 1.0).to(x.dtype)
+    x[:, ::3] = -0.0
+    x[:, 1::3] = 0.0
+    q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, w.to(DEV), 1e-6, fmt)
+    codes = q.cpu().view(torch.uint8) if fmt == "mxfp8" else R.unpack(q.cpu())
+    minus = 0x80 if fmt == "mxfp8" else 8
+    want = torch.where(torch.signbit(x.float() * w.float()), minus, 0).to(torch.uint8)
+    zero = x == 0
+    assert torch.equal(codes[zero], want[zero])
