@@ -189,6 +189,39 @@ __device__ __forceinline__ void mx_norm_pair(float* h, const float* w, uint64_t 
   for (int i = 0; i < 2; ++i) h[i] = __uint_as_float(__float_as_uint(out[i]) | (in[i] == out[i] ? 1u : 0u));
 }
 
+constexpr uint32_t kMaxBits = 0x7F7FFFFFu;  // float32's largest number
+
+// A span in which h w or y passes float32's range, or which holds infinities or
+// NaN, once more: from h times the power of two that takes sqrt(v) to about 1.
+// Its products pass the range only where y does; a y that reaches the largest
+// number counts as infinite. Apart, so that it takes no registers of the others.
+template <int kDt>
+__device__ __noinline__ void mx_norm_scaled(const uint8_t* hp, const uint8_t* wp, float hi, float lo0, float lo1, float* y) {
+  constexpr int kW = MxWords<kDt, 2>::n;
+  const uint32_t e = __float_as_uint(hi) >> 23;
+  const float down = __uint_as_float(e << 23), up = __uint_as_float((254u - e) << 23);  // hi up is in [1, 2)
+  hi *= up;
+  lo0 *= up;
+  lo1 *= up;
+#pragma unroll 1
+  for (int i = 0; i < kMxSpan; i += 2) {
+    uint32_t hw[kW], ww[kW];
+#pragma unroll
+    for (int k = 0; k < kW; ++k) {
+      hw[k] = reinterpret_cast<const volatile uint32_t*>(hp)[i / 2 * kW + k];
+      ww[k] = __ldg(reinterpret_cast<const uint32_t*>(wp) + i / 2 * kW + k);
+    }
+    float h[2], w[2];
+    mx_to_float<kDt>(hw, h);
+    mx_to_float<kDt>(ww, w);
+    h[0] *= down;
+    h[1] *= down;
+    mx_norm_pair<kDt>(h, w, f2_pack(hi, hi), f2_pack(lo0, lo0), f2_pack(lo1, lo1));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) y[i + k] = fabsf(h[k]) < __uint_as_float(kMaxBits) ? h[k] : h[k] + copysignf(INFINITY, h[k]);
+  }
+}
+
 constexpr int kNormPer = 2;  // spans of a thread
 
 // h = T(residual + x) (written back), y = h / sqrt(mean(h^2) + eps) * weight,
@@ -289,6 +322,7 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3)
     const uint32_t c = c0 + j * tpr;
     float f[kMxSpan];
     mx_to_float<kDt>(w[j], f);
+    uint32_t am;
     if (weight && live[j]) {
       uint32_t ww[kW];
       const uint4* wp = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(c) * kB);
@@ -305,8 +339,19 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3)
 #pragma unroll
       for (int i = 0; i < kMxSpan; i += 2)
         mx_norm_pair<kDt>(f + i, wf + i, f2_pack(hi, hi), f2_pack(lo0, lo0), f2_pack(lo1, lo1));
+      am = mx_span_max(f);
+      if (am >= kMaxBits && hi > 0.f) {
+        const uint8_t* hp = residual ? residual + row * res_ld_bytes : x + row * x_ld_bytes;
+        float again[kMxSpan];
+        mx_norm_scaled<kDt>(hp + static_cast<int64_t>(c) * kB, weight + static_cast<int64_t>(c) * kB, hi, lo0, lo1, again);
+#pragma unroll
+        for (int i = 0; i < kMxSpan; ++i) f[i] = again[i];
+        am = mx_span_max(f);
+      }
+    } else {
+      am = mx_span_max(f);
     }
-    const uint32_t am = mx_block_max<kFmt>(mx_span_max(f));
+    am = mx_block_max<kFmt>(am);
     uint32_t p[4];
     const uint32_t sc = mx_quant_span<kFmt>(f, am, gl, p);
     if (live[j]) mx_store_packed<kFmt>(q, scale, static_cast<uint64_t>(row) * per_row + c, p, sc);

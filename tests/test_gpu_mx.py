@@ -610,3 +610,34 @@ def test_norm_keeps_the_sign_of_zero(gpu_available, fmt, dtype, rows, cols):
     want = torch.where(torch.signbit(x.float() * w.float()), minus, 0).to(torch.uint8)
     zero = x == 0
     assert torch.equal(codes[zero], want[zero])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("cols", [64, 2048])
+def test_norm_whose_product_with_the_weight_is_large(gpu_available, fmt, dtype, cols):
+    """h w passes float32's range, y does not. One block has a y that does: its scale is NaN."""
+    dt = R.DTYPES[dtype]
+    g = _gen(60 + cols)
+    x = (torch.randn(5, cols, generator=g) * 1e15).to(dt)
+    x[1] *= 100.0
+    w = ((1 + 0.2 * torch.randn(cols, generator=g)) * 1e28).to(dt)
+    w[::7] = 1.0
+    w[40] = 2.0 ** 127
+    x[:, 40] = 0.0
+    x[2, 40] = 5e15
+    q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), None, w.to(DEV), 1e-5, fmt, *([torch.tensor([1e26], device=DEV)] if fmt == "nvfp4" else []))
+    h = x.double()
+    y = h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-5) * w.double()
+    over = (y.abs() > torch.finfo(torch.float32).max).view(5, -1, R.BLOCK[fmt]).any(-1)
+    assert over[2].any() and torch.equal(R.scale_values(s.cpu()).isnan(), over)
+    y[over.repeat_interleave(R.BLOCK[fmt], 1)] = 0.0
+    if fmt == "nvfp4":
+        v = R.values(q.cpu(), s.cpu(), fmt) * 1e26
+        ok = ~over.repeat_interleave(16, 1)
+        # half a step of e2m1 and the scale's 2^-4, as above
+        bound = y.abs() * (0.25 + 2.0 ** -4) + y.abs().view(5, -1, 16).amax(-1).repeat_interleave(16, 1) / 12
+        assert ((v - y).abs()[ok] <= bound[ok] * 1.01).all()
+    else:
+        ok = ~over.any(1)
+        _check_rows(fmt, q[ok.to(DEV)], s.view(torch.uint8)[ok.to(DEV)].view(s.dtype), y[ok])
