@@ -189,20 +189,46 @@ __device__ __forceinline__ void mx_norm_pair(float* h, const float* w, uint64_t 
   for (int i = 0; i < 2; ++i) h[i] = __uint_as_float(__float_as_uint(out[i]) | (in[i] == out[i] ? 1u : 0u));
 }
 
+// hi, lo0 and lo1 of inv = 1 / sqrt(v): the sum in v is within 2^-47, inv within 2^-48; lo
+// and its products add 2^-46. Neither lo is negative: the products of -0 stay -0.
+__device__ __forceinline__ float3 mx_root_bounds(double inv) {
+  const float hi = __double2float_rd(inv * (1.0 - 0x1p-41));
+  const float lo = static_cast<float>(inv - static_cast<double>(hi));
+  return make_float3(hi, lo - 0x1p-42f * hi, lo + 0x1p-42f * hi);
+}
+
+// The same where v is far from 1, whose reciprocal root may not be a float32:
+// that of v 4^e, with its sign turned for a sign, and 2^e in the place of lo1
+// (mx_norm_scaled multiplies h by it). Zero, infinite and NaN v: 1 / sqrt(v).
+__device__ __noinline__ float3 mx_far_root(double v) {
+  const double inv = 1.0 / sqrt(v);
+  if (!(v > 0.0 && v < INFINITY)) return make_float3(static_cast<float>(inv), 0.f, 0.f);
+  const int e = min((__double2hiint(inv) >> 20) - 1023, 127);  // -128 at least: v is below 2^256
+  const float3 r = mx_root_bounds(inv * __hiloint2double((1023 - e) << 20, 0));
+  return make_float3(-r.x, r.y, static_cast<float>(__hiloint2double((1023 + e) << 20, 0)));
+}
+
 constexpr uint32_t kMaxBits = 0x7F7FFFFFu;  // float32's largest number
 
-// A span in which h w or y passes float32's range, or which holds infinities or
-// NaN, once more: from h times the power of two that takes sqrt(v) to about 1.
+// A span in which h w or y passes float32's range, or of a row whose v is far
+// from 1 (mx_far_root): from h times the power of two that takes sqrt(v) to about 1.
 // Its products pass the range only where y does; a y that reaches the largest
 // number counts as infinite. Apart, so that it takes no registers of the others.
 template <int kDt>
 __device__ __noinline__ void mx_norm_scaled(const uint8_t* hp, const uint8_t* wp, float hi, float lo0, float lo1, float* y) {
   constexpr int kW = MxWords<kDt, 2>::n;
-  const uint32_t e = __float_as_uint(hi) >> 23;
-  const float down = __uint_as_float(e << 23), up = __uint_as_float((254u - e) << 23);  // hi up is in [1, 2)
-  hi *= up;
-  lo0 *= up;
-  lo1 *= up;
+  float down = lo1;
+  if (hi < 0.f) {  // from mx_far_root
+    hi = -hi;
+    lo1 = lo0 + 0x1p-41f * hi;
+  } else {
+    const uint32_t e = __float_as_uint(hi) >> 23;
+    const float up = __uint_as_float((254u - e) << 23);  // hi up is in [1, 2)
+    down = __uint_as_float(e << 23);
+    hi *= up;
+    lo0 *= up;
+    lo1 *= up;
+  }
 #pragma unroll 1
   for (int i = 0; i < kMxSpan; i += 2) {
     uint32_t hw[kW], ww[kW];
@@ -278,6 +304,7 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3)
     }
   }
   float hi = 1.f, lo0 = 0.f, lo1 = 0.f;
+  uint32_t again_at = kMaxBits;  // spans whose largest value has these bits or more go to mx_norm_scaled
   if (weight) {
     double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
@@ -296,24 +323,17 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3)
       for (uint32_t i = 0; i < blockDim.x / 32; ++i) ss += warp_ss[i];
     }
     const double v = ss / static_cast<double>(per_row * kMxSpan) + static_cast<double>(eps);
-    // 1 / sqrt(v): two Newton steps from the float32 estimate (2^-22, 2^-43,
-    // 2^-51) where that is an ordinary number, else the plain operations (zero
-    // rows, huge ones)
-    double inv;
     if (v > 1e-30 && v < 1e30) {
-      inv = static_cast<double>(rsqrtf(static_cast<float>(v)));
+      // two Newton steps from the float32 estimate: 2^-22, 2^-43, 2^-51
+      double inv = static_cast<double>(rsqrtf(static_cast<float>(v)));
 #pragma unroll
       for (int k = 0; k < 2; ++k) inv = fma(inv * fma(-v * inv, inv, 1.0), 0.5, inv);
+      const float3 r = mx_root_bounds(inv);
+      hi = r.x, lo0 = r.y, lo1 = r.z;
     } else {
-      inv = 1.0 / sqrt(v);
-    }
-    // the sum is within 2^-47, its root's reciprocal within 2^-48; lo and its products
-    // add 2^-46. Neither bound's lo is negative: the products of -0 stay -0
-    hi = __double2float_rd(inv * (1.0 - 0x1p-41));
-    if (hi < INFINITY) {
-      const float lo = static_cast<float>(inv - static_cast<double>(hi));
-      lo0 = lo - 0x1p-42f * hi;
-      lo1 = lo + 0x1p-42f * hi;
+      const float3 r = mx_far_root(v);
+      hi = r.x, lo0 = r.y, lo1 = r.z;
+      again_at = hi < 0.f ? 0u : 0xFFFFFFFFu;
     }
   }
   const MxGlobal gl = mx_global(kFmt == kFmtNvfp4 ? global_scale : nullptr);
@@ -340,7 +360,7 @@ __global__ void __launch_bounds__(kMaxT, kMaxT == 256 ? (kDt != kDtFp32 ? 5 : 3)
       for (int i = 0; i < kMxSpan; i += 2)
         mx_norm_pair<kDt>(f + i, wf + i, f2_pack(hi, hi), f2_pack(lo0, lo0), f2_pack(lo1, lo1));
       am = mx_span_max(f);
-      if (am >= kMaxBits && hi > 0.f) {
+      if (am >= again_at) {
         const uint8_t* hp = residual ? residual + row * res_ld_bytes : x + row * x_ld_bytes;
         float again[kMxSpan];
         mx_norm_scaled<kDt>(hp + static_cast<int64_t>(c) * kB, weight + static_cast<int64_t>(c) * kB, hi, lo0, lo1, again);

@@ -232,7 +232,8 @@ def add_rmsnorm_quantize_mx(x: torch.Tensor, residual: torch.Tensor | None = Non
     microscaled formats: ``h = residual + x`` rounded to x's type (written back
     into ``residual``), ``y = h / sqrt(mean(h^2) + eps) * norm_weight``, then
     the quantisation of y as in ``quantize_mx`` (y is rounded to odd in float32,
-    so a value lands where the exact y would). ``residual`` None: h = x;
+    so a value lands where the exact y would; the mean is taken in float64, so h
+    may have any size; a y of float32's largest number or more counts as infinite). ``residual`` None: h = x;
     ``norm_weight`` None: y = h. All three tensors have x's type. Returns
     (packed values, scales)."""
     f = _format(fmt)

@@ -301,7 +301,7 @@ int moe_fp8_ds_dequantize_mx(const void* q, const void* scale, int64_t rows, int
  * width up to 32768 (moe_fp8_ds_add_norm_quant is the 7168-wide form with
  * 1x128 fp32 scales):
  *   h = dtype(residual + x)                    written back to residual
- *   y = h / sqrt(mean(h^2) + eps) * weight     in float32
+ *   y = h / sqrt(mean(h^2) + eps) * weight     in float32 (rounded to odd), the mean in float64
  *   q_out, scale_out = the quantisation of y
  * residual NULL: h = x. norm_weight (dtype, [cols]) NULL: y = h.
  */

@@ -641,3 +641,29 @@ def test_norm_whose_product_with_the_weight_is_large(gpu_available, fmt, dtype, 
     else:
         ok = ~over.any(1)
         _check_rows(fmt, q[ok.to(DEV)], s.view(torch.uint8)[ok.to(DEV)].view(s.dtype), y[ok])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,cols", [(5, 32), (7, 96), (6, 512), (3, 7168)])
+def test_norm_of_very_large_and_very_small_rows(gpu_available, fmt, dtype, rows, cols):
+    """Squares that pass float32's range or fall below it, beside ordinary rows."""
+    dt = R.DTYPES[dtype]
+    g = _gen(rows + cols)
+    w = (1 + 0.2 * torch.randn(cols, generator=g)).to(dt)
+    for size, eps in ((1e20, 1e-5), (3e37, 1e-5), (1e-22, 0.0), (1e-30, 0.0), (1e-36, 1e-30), (1e-39, 0.0)):
+        x = torch.randn(rows, cols, generator=g)
+        x[::2] *= size
+        x = x.to(dt)
+        res = torch.zeros_like(x).to(DEV)
+        q, s = pkg().add_rmsnorm_quantize_mx(x.to(DEV), res, w.to(DEV), eps, fmt)
+        assert torch.equal(res.cpu(), x)
+        h = x.double()
+        e = float(torch.tensor(eps, dtype=torch.float32))
+        y = h / torch.sqrt(h.square().mean(1, keepdim=True) + e) * w.double()
+        if fmt == "nvfp4":
+            # amax / 6 below 2^-10, half of e4m3's smallest number, is a scale of 0 and zeros: y ~ 1e-21 of size 1e-36
+            none = y.view(rows, -1, 16).abs().amax(-1) / 6 < 2.0 ** -10 * (1 - 2.0 ** -16)
+            assert (s.cpu().float()[none] == 0).all() and (R.unpack(q.cpu()).view(rows, -1, 16)[none] == 0).all()
+            y[none.repeat_interleave(16, 1)] = 0.0
+        _check_rows(fmt, q, s, y)
