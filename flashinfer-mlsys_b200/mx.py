@@ -17,16 +17,21 @@ mxfp8; scales are ``torch.float8_e4m3fn [rows, cols / 16]`` (nvfp4) or
 Every call runs in ``libmoe_fp8_ds.so`` on the current CUDA stream of the
 tensors' device, keeps no state and needs no workspace, so calls may overlap
 on different streams and be captured into CUDA graphs. There is no fallback:
-bad arguments raise ``ValueError``, a failing call raises ``MoeError``.
+bad arguments raise ``ValueError``, a failing call raises ``MoeError``. None of
+them is differentiable: results carry no gradient, and a tensor that a call has
+written cannot be used by an earlier graph's backward pass. Outputs must not
+share memory with other arguments.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .binding import _stream
 
 _Tensor = torch.Tensor
+_current_device = torch._C._cuda_getDevice
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
 
@@ -54,13 +59,20 @@ def _bad(msg):
 def _run(dev, name, *args):
     """Calls a C-ABI function with `dev` current on its current stream."""
     fn = getattr(_lib._lib or _lib.load(), name)
-    if dev.index == torch._C._cuda_getDevice():
+    if dev.index == _current_device():
         rc = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _stream(dev))
     if rc:
         _lib.check(rc, name)
+
+
+def _wrote(t):
+    """Counts a version of a tensor of the caller's that a call has written, so
+    that autograd refuses a backward pass that would read it as it was (0.3 us)."""
+    if t is not None and not t.is_inference():
+        increment_version(t)
 
 
 def _format(fmt):
@@ -186,9 +198,12 @@ def quantize_mx(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor 
     rows, cols = x.shape
     _size(rows, cols)
     g = _global_scale(global_scale, fmt, dev)
+    given, given_scale = out, out_scale
     out, out_scale, qp, sp = _packed_out(rows, cols, f, dev, out, out_scale)
     if rows:
         _run(dev, "moe_fp8_ds_quantize_mx", x.data_ptr(), code, rows, cols, ld, f[0], g, qp, sp)
+        _wrote(given)
+        _wrote(given_scale)
     return out, out_scale
 
 
@@ -212,6 +227,7 @@ def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, fmt: str = "nvfp4", glob
     dev = _cuda(q, "q")
     rows, cols, qp, sp = _packed_in(q, scale, f, dev, ("q", "scale"))
     g = _global_scale(global_scale, fmt, dev)
+    given = out
     if out is None:
         code, ld = _DTYPES.get(dtype), cols
         if code is None:
@@ -221,6 +237,7 @@ def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, fmt: str = "nvfp4", glob
         code, ld = _matrix(out, "out", dev, None, (rows, cols))
     if rows:
         _run(dev, "moe_fp8_ds_dequantize_mx", qp, sp, rows, cols, f[0], g, code, out.data_ptr(), ld)
+        _wrote(given)
     return out
 
 
@@ -251,9 +268,13 @@ def add_rmsnorm_quantize_mx(x: torch.Tensor, residual: torch.Tensor | None = Non
     if norm_weight is not None:
         wp = _exact16(norm_weight, "norm_weight", x.dtype, (cols,), dev)
     g = _global_scale(global_scale, fmt, dev)
+    given, given_scale = out, out_scale
     out, out_scale, qp, sp = _packed_out(rows, cols, f, dev, out, out_scale)
     if rows:
         _run(dev, "moe_fp8_ds_add_norm_quantize_mx", x.data_ptr(), ld, rp, rld, wp, eps, code, rows, cols, f[0], g, qp, sp)
+        _wrote(residual)
+        _wrote(given)
+        _wrote(given_scale)
     return out, out_scale
 
 
@@ -299,9 +320,11 @@ def matmul_mx(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     n, kb, bp, bsp = _packed_in(b, b_scale, f, dev, ("b", "b_scale"))
     _same_width(k, kb, m, n)
     al = _scalar(alpha, "alpha", dev)
+    given = out
     out, code, ld = _product_out(m, n, dev, out, out_dtype, torch.empty)
     if m:
         _run(dev, "moe_fp8_ds_matmul_mx", ap, asp, bp, bsp, m, n, k, f[0], al, out.data_ptr(), code, ld)
+        _wrote(given)
     return out
 
 
@@ -328,7 +351,9 @@ def experts_matmul_mx(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b
     _same_width(k, kb, m, n)
     op = _exact(expert_offsets, "expert_offsets", torch.int32, (e + 1,), dev)
     al = None if alpha is None else _exact(alpha, "alpha", torch.float32, (e,), dev)
+    given = out
     out, code, ld = _product_out(m, n, dev, out, out_dtype, torch.zeros)
     if m:
         _run(dev, "moe_fp8_ds_experts_matmul_mx", ap, asp, bp, bsp, op, e, m, n, k, f[0], al, out.data_ptr(), code, ld)
+        _wrote(given)
     return out

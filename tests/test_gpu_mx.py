@@ -667,3 +667,25 @@ def test_norm_of_very_large_and_very_small_rows(gpu_available, fmt, dtype, rows,
             assert (s.cpu().float()[none] == 0).all() and (R.unpack(q.cpu()).view(rows, -1, 16)[none] == 0).all()
             y[none.repeat_interleave(16, 1)] = 0.0
         _check_rows(fmt, q, s, y)
+
+
+def test_written_tensors_are_known_to_autograd(gpu_available):
+    """A tensor that autograd has saved and a call then writes: the backward
+    pass refuses, as after any other write in place."""
+    m = pkg()
+    x = torch.randn(4, 64, generator=_gen(70)).to(DEV)
+    q, s = m.quantize_mx(x, "mxfp8")
+    leaf = torch.randn(4, 64, generator=_gen(71)).to(DEV).requires_grad_(True)
+    for write in (lambda t: m.add_rmsnorm_quantize_mx(x, t, None), lambda t: m.dequantize_mx(q, s, "mxfp8", out=t),
+                  lambda t: m.matmul_mx(q, s, torch.cat([q.view(torch.uint8)] * 16).view(q.dtype),
+                                        torch.cat([s.view(torch.uint8)] * 16).view(s.dtype), "mxfp8", out=t)):
+        t = leaf * 2.0
+        loss = (t * t).sum()
+        with torch.no_grad():
+            write(t)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():  # tensors without a version are written all the same
+        t = x * 1.0
+        m.dequantize_mx(q, s, "mxfp8", out=t)
+        assert torch.equal(t.cpu(), R.values(q.cpu(), s.cpu(), "mxfp8").float())
