@@ -689,3 +689,46 @@ def test_written_tensors_are_known_to_autograd(gpu_available):
         t = x * 1.0
         m.dequantize_mx(q, s, "mxfp8", out=t)
         assert torch.equal(t.cpu(), R.values(q.cpu(), s.cpu(), "mxfp8").float())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_weighted_sum_of_the_experts_rows(gpu_available, fmt):
+    """The chain of the test above, with its final output: token by token, slot
+    by slot in float64 from the quantised values and the routing, without the
+    sort and the offsets."""
+    m = pkg()
+    T, H, I, E = 24, 512, 256, 32
+    g = _gen(43)
+    x, res = (torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(H, generator=g)).to(torch.bfloat16).to(DEV)
+    logits = torch.randn(T, 256, generator=g).to(DEV)
+    ids, wts, n = m.route(logits, torch.zeros(256, dtype=torch.bfloat16, device=DEV), 0, E, 2.5)
+    flat = ids.flatten()
+    order = torch.argsort(torch.where(flat < E, flat, E), stable=True)[: int((flat < E).sum())]
+    tok = order // 8
+    off = torch.cat((n.new_zeros(1), n[:E].cumsum(0))).int()
+    q, s = m.add_rmsnorm_quantize_mx(x, res, w, 1e-6, fmt)
+    w13, s13 = (t.to(DEV) for t in R.random_packed(g, (E,), I, H, fmt))
+    w2, s2 = (t.to(DEV) for t in R.random_packed(g, (E,), H, I, fmt))
+    h = m.experts_matmul_mx(q[tok].contiguous(), s.view(torch.uint8)[tok].contiguous().view(s.dtype), w13, s13, off, fmt)
+    qi, si = m.quantize_mx(h, fmt)
+    y = m.experts_matmul_mx(qi, si, w2, s2, off, fmt, out_dtype=torch.float32)
+    out = torch.zeros(T, H, device=DEV).index_add_(0, tok, y * wts.flatten()[order][:, None]).cpu().double()
+    assert m.device_status() == 0
+    a, up, down = R.values(q.cpu(), s.cpu(), fmt), R.values(w13.cpu(), s13.cpu(), fmt), R.values(w2.cpu(), s2.cpu(), fmt)
+    hv, yv, wv = h.cpu().double(), R.values(qi.cpu(), si.cpu(), fmt), wts.cpu().double()
+    row = {int(o): i for i, o in enumerate(order.tolist())}  # slot -> sorted row
+    want, size = torch.zeros(T, H, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
+    for t in range(T):
+        for k in range(8):
+            e = int(ids[t, k])
+            if e >= E:
+                continue
+            i = row[8 * t + k]
+            mag = a[t].abs() @ up[e].abs().t()
+            assert ((hv[i] - a[t] @ up[e].t()).abs() <= (H / 32 + 8) * 2.0 ** -23 * mag + 2.0 ** -8 * 1.01 * hv[i].abs() + 1e-30).all()
+            want[t] += wv[t, k] * (yv[i] @ down[e].t())
+            size[t] += wv[t, k] * (yv[i].abs() @ down[e].abs().t())
+    assert (size.amax(1) > 0).sum() > T // 2
+    # the product's steps as in _product_ok, then a product and at most eight additions of 2^-24
+    assert ((out - want).abs() <= ((I / 32 + 8) * 2.0 ** -23 + 10 * 2.0 ** -24) * size + 1e-30).all()
