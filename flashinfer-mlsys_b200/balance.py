@@ -78,9 +78,11 @@ def balance_loss(routing_logits: torch.Tensor, topk_ids: torch.Tensor, seq_offse
 
     Returns (loss float32 [S], counts int32 [S, E]). Scores are within 5
     float32 steps of the exact ones (softmax: for the float32 difference to the
-    row's largest logit). An empty sequence has loss 0; tokens of no sequence count nowhere and get a zero gradient; a token
-    whose scores vanish in float32 (sigmoids of logits under -87) has p = 0. ``counts.sum(0)`` is what a
-    bias update of the no-aux router needs."""
+    row's largest logit). An empty sequence has loss 0; tokens of no sequence
+    count nowhere and get a zero gradient; a token whose scores vanish in float32
+    (sigmoids of logits under -87) has p = 0. Offsets that decrease give undefined
+    numbers, not an access out of range. ``counts.sum(0)`` is what a bias update of
+    the no-aux router needs."""
     dev = _cuda(routing_logits, "routing_logits")
     _cuda(topk_ids, "topk_ids")
     if routing_logits.dim() != 2 or topk_ids.dim() != 2:

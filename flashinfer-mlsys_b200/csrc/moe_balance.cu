@@ -8,9 +8,9 @@
 //   p_ti = a_ti / sum_j a_tj,   P_i = 1/T_s sum_t p_ti
 //   loss_s = coeff * sum_i f_i P_i
 //   d loss_s / d l_tj = coeff / T_s * p_tj (f_j - sum_i f_i p_ti) * (1 - sigmoid(l_tj) for sigmoid, 1 for exp)
-// An empty sequence has loss 0; a token whose scores sum to zero (every logit
-// -inf) has p = 0 and no gradient; ids outside [0, E) are not counted; tokens
-// of no sequence get a zero gradient.
+// An empty sequence has loss 0; a token whose float32 scores sum to zero (every
+// logit -inf, or under -87 for sigmoids) has p = 0 and no gradient; ids outside
+// [0, E) are not counted; tokens of no sequence get a zero gradient.
 //
 // HBM-bound: one pass over the logits forward, one (and the gradient) back.
 // Forward: CTAs own equal runs of tokens, whatever the sequences' lengths. A
@@ -19,8 +19,8 @@
 // segment's fp32 column sums and counts go to a slot of their own. A second
 // kernel adds a sequence's slots in order. No atomics on floats: results do
 // not depend on the order in which CTAs run. 65536 x 256 fp32 in 13 sequences:
-// forward 20.5 us (3.3 TB/s), backward 26.9 us (5.0 TB/s); 16384 x 256: 11.0 and
-// 10.0 us, of which launches and dependent loads are the most.
+// forward 22.8 us (2.9 TB/s), backward 28.9 us (4.6 TB/s); 16384 x 256: 11.5 and
+// 10.7 us, of which launches and dependent loads are the most.
 #include "moe_kernels.h"
 
 namespace moe {
@@ -107,7 +107,9 @@ struct BalArgs {
   float coeff;
 };
 
-// Sequence bounds, kept inside [0, T] and in order whatever `off` holds.
+// Sequence bounds, kept inside [0, T], and the end not before the start. Offsets
+// that decrease from one sequence to the next are not put in order: sequences
+// then overlap, may share a slot and have no defined sums, inside their bounds.
 __device__ __forceinline__ void bal_bounds(const BalArgs& a, int s, int64_t* lo, int64_t* hi) {
   if (!a.off) {
     *lo = 0;

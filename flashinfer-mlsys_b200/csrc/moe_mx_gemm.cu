@@ -36,9 +36,9 @@
 //   32 experts x 7168 x 4096 nvfp4, 64 rows   71 us, 6.3 TB/s: HBM (27 experts
 //     with rows; 28 are 79 us, as their tiles are 6.05 waves of CTAs)
 //   32 experts x 2048 x 7168 mxfp4, 8192 rows 87 us, 4.3 TB/s: eight stages a
-//     tile, in which neither HBM (55%) nor the tensor pipe (34%) is kept busy;
+//     tile, in which neither HBM (45% by its counter) nor the tensor pipe (34%) is kept busy;
 //     the MMA issuer waits in turn for tiles, scales and accumulators
-//   8 x 7168 x 4096 nvfp4       7.2 us: launch, one exchange across the
+//   8 x 7168 x 4096 nvfp4       7.4 us: launch, one exchange across the
 //     cluster and some 2.6 us of weights
 #include <atomic>
 #include <type_traits>
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
     }
   } else if (warp < kMxSfWarp0 + kMxSfWarps) {
     // ======================= scale loaders =======================
-    // Four stages at a time into one of two slots: lane 8 j + r of warp b
+    // Four stages at a time into the next slot (of two, three or four): lane 8 j + r of warp b
     // loads stage j's words of rows 8 b + r, + 32, + 64, + 96 of every
     // 128-row group (four lanes read a row's neighbouring words) and stores
     // each word's four rows as one 16-byte piece.
@@ -748,9 +748,10 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       } else if (u_first < units) {
         // A CTA by itself streams weights, whose scales come from HBM: the next
         // group's loads start before this one's are waited for. 32 experts x
-        // 7168 x 4096 nvfp4, 64 rows on 27 of them: 74.2 -> 70.9 us. (A split has a group or
-        // two and loses 4% to the longer code; in a pair both groups' words do
-        // not fit the registers, and a group takes longer to use than to load.)
+        // 7168 x 4096 nvfp4, 64 rows on 27 of them: 74.2 -> 70.9 us; the longer code costs
+        // calls of 8 and of 128 rows 1 to 2%. (A split has a group or two and loses 4%.
+        // In a pair two groups of nvfp4 are 96 words a lane, which do not fit the
+        // registers; mxfp4's 48 and mxfp8's 24 would, and were not tried.)
         MxUnit xa = mx_unit(ctl, p, u_first, ntn, kTileRows), xb = xa;
         int u = u_first, ka = k0, kb = k0;
         uint32_t wa[1 + Cfg::kChunks][4][kR], wb[1 + Cfg::kChunks][4][kR];
@@ -957,7 +958,10 @@ cudaError_t mx_gemm_launch_nt(const MxPlan& pl, const CUtensorMap& mw, const CUt
 // Several runs, whose lengths only the device knows: by their mean length. 32
 // x 7168 x 4096 nvfp4: at a mean of 32 rows tiles of 64 take 94 us and pairs of
 // 256 102 us, at 64 rows 142 and 104 us, at 128 rows tiles of 128 149 us and
-// pairs 111 us.
+// pairs 111 us. All of even runs over many weight rows; the rule knows neither
+// N nor the number of tiles. Few experts with small N get pairs that leave most
+// SMs idle, and short runs that are far from even (256 rows, all of one of 32
+// experts) get narrow tiles that load the weights again and again.
 // Token rows of a copy where the runs' lengths are known to the device only: a
 // short tile then loads little more than it has.
 constexpr int kMxRunBox = 64;

@@ -6,8 +6,8 @@
 // (the norm 149 -> 142 us with nvfp4, 140 -> 136 us with mxfp8), fp32 rows
 // would spill (233 -> 354 us) and keep three CTAs (two: 140 us at 8192 rows, not 119). At 16384 x 7168 bf16: quantisation 54 us nvfp4
 // (5.5 TB/s; some 12 instructions a value nearly bind), 46 us mxfp4, 52 us mxfp8
-// (6.8 TB/s), dequantisation 45 us (6.6 TB/s), residual + norm + mxfp8 136 us
-// (6.1 TB/s); fp32 rows 6.3 to 7.1 TB/s.
+// (6.8 TB/s), dequantisation 45 us (6.6 TB/s), residual + norm + mxfp8 134 us
+// (6.1 TB/s), nvfp4 144 us; fp32 rows 6.3 to 7.1 TB/s.
 #include "moe_kernels.h"
 #include "moe_mx.cuh"
 
